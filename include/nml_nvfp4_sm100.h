@@ -586,6 +586,127 @@ int32_t nml_sm100_paged_attention_decode(const NmlSm100PagedAttentionDecode *req
 size_t nml_sm100_paged_attention_decode_workspace_bytes(int64_t batch, int64_t query_heads,
                                                         int64_t splits);
 
+/* ---- 8-bit paged K/V cache -------------------------------------------------------------------
+ * The cache of the paged attention above at half its bytes: keys and values as E4M3 codes with
+ * one power-of-two scale for every block of one page (16 tokens) and one kv head,
+ *   codes   u8 [physical_pages, kv_heads, page_size, head_dim]
+ *   scales  u8 [physical_pages, kv_heads], E8M0: value = e4m3(code) * 2^(scale - 127)
+ * so that a block is contiguous (1 or 2 KB).  Not part of the reference: its caches hold 16-bit
+ * values (crates/nml-ir/src/lib.rs:4717-4730).  Limits: head_dim 64 or 128, page_size 16.
+ *
+ * Quantisation: the exponent of a block is the smallest e in [-48, 48] with |x| <= 448 * 2^e for
+ * every finite row written to it, codes round to nearest even, larger magnitudes saturate.  A
+ * token's row of one head that holds an infinity or a NaN is stored as NaN codes throughout.
+ * Powers of two cost an 8-bit float no precision, and make a block's values exact in 16 bits.
+ *
+ * Slots that no token was written to may hold anything; a page may be shared by sequences (a
+ * common prefix) as long as none of them writes to it.  Page table entries outside
+ * [0, physical_pages) and lengths beyond table_width pages raise NML_SM100_STATUS_INDEX_RANGE;
+ * the tokens concerned are neither written nor visible. */
+typedef struct NmlSm100CacheQ8 {
+  uint8_t *key;                    /* codes, 16-byte aligned */
+  uint8_t *key_scales;
+  uint8_t *value;                  /* codes, 16-byte aligned */
+  uint8_t *value_scales;
+  const int32_t *page_table;       /* [batch, table_width] */
+  const int32_t *sequence_lengths; /* [batch], 0 for an empty place; not read by the read-back */
+  int64_t batch;
+  int64_t kv_heads;
+  int64_t head_dim;
+  int64_t page_size;
+  int64_t physical_pages;
+  int64_t table_width;
+} NmlSm100CacheQ8;
+
+/* Rotary positions and the cache write in one launch.  The rows of sequence b are
+ * [token_offsets[b], token_offsets[b + 1]) (one row each when token_offsets is NULL), its last
+ * tokens: row i of n has position sequence_lengths[b] - n + i.  Keys are rotated in f32 and
+ * rounded once, to their codes; values are only quantised; `query`, when given, is rotated into
+ * query_output.  Rows at a negative position (an empty place of a padded batch) write nothing to
+ * the cache and give zero query rows; rows outside every sequence are left as they were.
+ *
+ * A block that already holds older tokens of the sequence keeps their scale as a lower bound; when
+ * the new rows need a larger one, the older codes are rounded again to it.
+ *
+ * rotary: f32 [rotary_rows, rotary_dim], cosines then sines of every position (scaled as the model
+ * scales its long contexts); rotates the first rotary_dim (a multiple of 16) elements of every
+ * head, as pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved.  NULL: no rotation.
+ * A position at or past rotary_rows raises NML_SM100_STATUS_INDEX_RANGE and is handled as a
+ * negative one.  Strides are in elements, multiples of 8; rows of a head are contiguous and
+ * 16-byte aligned.  query_output must not overlap the inputs. */
+typedef struct NmlSm100PagedAppendQ8 {
+  size_t struct_size;
+  NmlSm100CacheQ8 cache;
+  const void *key;                 /* [tokens, kv_heads, head_dim] dtype */
+  const void *value;               /* [tokens, kv_heads, head_dim] dtype */
+  const void *query;               /* [tokens, query_heads, head_dim] dtype or NULL */
+  void *query_output;              /* same shape; NULL without query */
+  const int32_t *token_offsets;    /* [batch + 1] or NULL (then tokens == batch) */
+  const float *rotary;             /* [rotary_rows, rotary_dim] or NULL */
+  void *stream;
+  int64_t tokens;
+  int64_t query_heads;
+  int64_t key_token_stride, key_head_stride;
+  int64_t value_token_stride, value_head_stride;
+  int64_t query_token_stride, query_head_stride;
+  int64_t output_token_stride, output_head_stride;
+  int64_t rotary_rows;
+  int64_t rotary_dim;
+  int32_t rotary_interleaved;
+  int32_t dtype;
+} NmlSm100PagedAppendQ8;
+int32_t nml_sm100_paged_append_q8(const NmlSm100PagedAppendQ8 *request, char *error_message,
+                                  size_t error_message_capacity);
+
+/* Reads the first token_offsets[b + 1] - token_offsets[b] tokens of every sequence back as 16-bit
+ * values into rows [token_offsets[b], token_offsets[b + 1]) of the outputs; rows outside every
+ * sequence are left as they were, rows behind a bad page table entry become zeros. */
+typedef struct NmlSm100PagedReadQ8 {
+  size_t struct_size;
+  NmlSm100CacheQ8 cache;
+  const int32_t *token_offsets;    /* [batch + 1] */
+  void *key_output;                /* [tokens, kv_heads, head_dim] dtype */
+  void *value_output;              /* [tokens, kv_heads, head_dim] dtype */
+  void *stream;
+  int64_t tokens;
+  int32_t dtype;
+} NmlSm100PagedReadQ8;
+int32_t nml_sm100_paged_read_q8(const NmlSm100PagedReadQ8 *request, char *error_message,
+                                size_t error_message_capacity);
+
+/* Attention over the 8-bit cache, for single tokens (query_offsets NULL: one query of every
+ * sequence, at its last token) and for ragged runs of tokens (prompts, chunks of them, drafted
+ * tokens): rows [query_offsets[b], query_offsets[b + 1]) are the last tokens of sequence b, as in
+ * the append.  Token j is visible at position i when j <= i and, with a sliding window,
+ * j > i - sliding_window or j < first_tokens.  `sinks` as in the 16-bit operator.  A row that sees
+ * nothing becomes zeros; rows outside every sequence are left as they were.  Scores, softmax
+ * statistics and sums are f32; queries of BF16 are narrowed to F16 after a power of two for every
+ * row that makes this exact down to 2^-29 of the row's largest; probabilities are narrowed to F16. */
+typedef struct NmlSm100PagedAttentionQ8 {
+  size_t struct_size;
+  NmlSm100CacheQ8 cache;
+  const void *query;               /* [tokens, query_heads, head_dim] dtype */
+  const int32_t *query_offsets;    /* [batch + 1] or NULL (then tokens == batch) */
+  const float *sinks;              /* [query_heads] f32 or NULL */
+  void *output;                    /* [tokens, query_heads, head_dim] dtype, contiguous */
+  void *workspace;                 /* 16-byte aligned, may be NULL when 0 bytes are asked for */
+  size_t workspace_bytes;
+  void *stream;
+  int64_t tokens;
+  int64_t query_heads;             /* a multiple of kv_heads, at most 128 for each of them */
+  int64_t query_token_stride, query_head_stride; /* elements, multiples of 8 */
+  int64_t sliding_window;          /* 0: none */
+  int64_t first_tokens;            /* tokens in front that stay visible past the window */
+  int64_t splits;                  /* parts of a sequence's tokens, 1..64; 0: the library's choice */
+  float scale;                     /* softmax scale, usually head_dim^-0.5 */
+  int32_t dtype;
+} NmlSm100PagedAttentionQ8;
+int32_t nml_sm100_paged_attention_q8(const NmlSm100PagedAttentionQ8 *request,
+                                     char *error_message, size_t error_message_capacity);
+/* Scratch bytes of the call that `request` describes (its pointers are not read); the scratch
+ * carries nothing from one call to the next. */
+size_t nml_sm100_paged_attention_q8_workspace_bytes(const NmlSm100PagedAttentionQ8 *request);
+
 /* Routed clamped-SwiGLU layer for callers that cannot hand over scratch memory.
  *
  * This entry point has no counterpart in the reference.  Some hosts of this library have

@@ -151,6 +151,40 @@ class PagedAttentionDecode(ctypes.Structure):
                 ("dtype", _i32)]
 
 
+class CacheQ8(ctypes.Structure):
+    _fields_ = [("key", _vp), ("key_scales", _vp), ("value", _vp), ("value_scales", _vp),
+                ("page_table", _vp), ("sequence_lengths", _vp), ("batch", _i64),
+                ("kv_heads", _i64), ("head_dim", _i64), ("page_size", _i64),
+                ("physical_pages", _i64), ("table_width", _i64)]
+
+
+class PagedAppendQ8(ctypes.Structure):
+    _fields_ = [("struct_size", _sz), ("cache", CacheQ8), ("key", _vp), ("value", _vp),
+                ("query", _vp), ("query_output", _vp), ("token_offsets", _vp), ("rotary", _vp),
+                ("stream", _vp), ("tokens", _i64), ("query_heads", _i64),
+                ("key_token_stride", _i64), ("key_head_stride", _i64),
+                ("value_token_stride", _i64), ("value_head_stride", _i64),
+                ("query_token_stride", _i64), ("query_head_stride", _i64),
+                ("output_token_stride", _i64), ("output_head_stride", _i64),
+                ("rotary_rows", _i64), ("rotary_dim", _i64), ("rotary_interleaved", _i32),
+                ("dtype", _i32)]
+
+
+class PagedReadQ8(ctypes.Structure):
+    _fields_ = [("struct_size", _sz), ("cache", CacheQ8), ("token_offsets", _vp),
+                ("key_output", _vp), ("value_output", _vp), ("stream", _vp), ("tokens", _i64),
+                ("dtype", _i32)]
+
+
+class PagedAttentionQ8(ctypes.Structure):
+    _fields_ = [("struct_size", _sz), ("cache", CacheQ8), ("query", _vp), ("query_offsets", _vp),
+                ("sinks", _vp), ("output", _vp), ("workspace", _vp), ("workspace_bytes", _sz),
+                ("stream", _vp), ("tokens", _i64), ("query_heads", _i64),
+                ("query_token_stride", _i64), ("query_head_stride", _i64),
+                ("sliding_window", _i64), ("first_tokens", _i64), ("splits", _i64),
+                ("scale", ctypes.c_float), ("dtype", _i32)]
+
+
 class RoutedWorkspaceLayout(ctypes.Structure):
     _fields_ = [("sorted_assignments", _sz), ("block_experts", _sz), ("active_blocks", _sz),
                 ("activated", _sz), ("weighted", _sz), ("permuted_hidden", _sz),
@@ -224,6 +258,9 @@ REQUEST_ENTRY_POINTS = {
     "nml_nvfp4_sm100_combine_rows": CombineRows,
     "nml_sm100_paged_attention_decode": PagedAttentionDecode,
     "nml_nvfp4_sm100_topk_rows": TopkRows,
+    "nml_sm100_paged_append_q8": PagedAppendQ8,
+    "nml_sm100_paged_read_q8": PagedReadQ8,
+    "nml_sm100_paged_attention_q8": PagedAttentionQ8,
 }
 
 OTHER_ENTRY_POINTS = [
@@ -239,6 +276,7 @@ OTHER_ENTRY_POINTS = [
     "nml_nvfp4_sm100_abi_version",
     "nml_sm100_paged_attention_decode_workspace_bytes",
     "nml_nvfp4_sm100_topk_rows_workspace_bytes",
+    "nml_sm100_paged_attention_q8_workspace_bytes",
 ]
 
 
@@ -281,6 +319,9 @@ def load() -> ctypes.CDLL:
     lib.nml_nvfp4_sm100_topk_rows_workspace_bytes.argtypes = [_i64] * 3
     lib.nml_sm100_paged_attention_decode_workspace_bytes.restype = _sz
     lib.nml_sm100_paged_attention_decode_workspace_bytes.argtypes = [_i64] * 3
+    lib.nml_sm100_paged_attention_q8_workspace_bytes.restype = _sz
+    lib.nml_sm100_paged_attention_q8_workspace_bytes.argtypes = [
+        ctypes.POINTER(PagedAttentionQ8)]
     lib.nml_nvfp4_sm100_plan_capacity.restype = _i32
     lib.nml_nvfp4_sm100_plan_capacity.argtypes = [_i64, _i64, ctypes.POINTER(_i64),
                                                   ctypes.POINTER(_i64)]

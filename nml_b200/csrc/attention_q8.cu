@@ -1,0 +1,596 @@
+// Attention over the 8-bit paged K/V cache, one query row (token) at a time: the form for single
+// tokens, bound by reading every visible code once.
+//
+//   out = sum_j p_j v_j / (sum_j p_j + exp(sink)),  p_j = exp(scale * q.k_j)
+//
+// With k_j = 2^a code_j and v_j = 2^b code'_j (one exponent for each block of 16 tokens) both
+// products run on the bare codes, which are exact in f16:
+//
+//   t_j = q.code_j * (scale log2(e) 2^a),   w_j = exp2(t_j + b - M),   M = max_j (t_j + b)
+//   numerator = sum_j w_j code'_j,          denominator = sum_j w_j 2^-b
+//
+// so a block's scales cost one factor of the scores and one addend of the exponent, and M bounds
+// what actually enters the f16 product.  The exponents lie in [-48, 48]: a weight that underflows
+// (w_j < 2^-126) is below 2^-24 of the denominator's largest term.
+//
+// Shape of the work: one CTA per (row, kv head and up to 16 of its query heads, split of the
+// visible pages); its warps take chunks of pages in turn.  A block is 16 * head_dim contiguous
+// bytes, loaded straight into mma.sync fragments by 16-byte (keys) and 8- or 16-byte (values)
+// loads, the next chunk's while this one is worked on: scores [16 tokens x 8 heads] = K . q^T, the
+// weights transposed between lanes by movmatrix, out^T [dims x 8 heads] += V^T . w, where pairs of
+// tokens are interleaved byte-wise before they are widened.
+#include <type_traits>
+
+#include "cache_q8.cuh"
+
+namespace nml_sm100 {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct AttentionParams {
+  CacheQ8 cache;
+  const void* query;
+  const int32_t* offsets;  // [batch + 1] or null
+  const float* sinks;
+  float* partial;          // [rows, query_heads, splits, D + 2]: out, maximum, sum
+  void* output;
+  int64_t query_token_stride, query_head_stride;
+  int tokens, query_heads, group, head_tiles, splits, window, first;
+  float scale_log2;
+  int* status;
+};
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 8x8 16-bit transpose between lanes: row r of the input is held by lanes 4r .. 4r + 3.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
+// Which logical pages a row sees: [0, front) and [back, end), and its token limits.
+struct Visible {
+  int length;  // tokens in front of (and with) the row's own
+  int start;   // first token of the window
+  int front, back, pages;
+};
+
+__device__ __forceinline__ Visible visible_pages(int length, int window, int first) {
+  Visible v;
+  v.length = max(length, 0);
+  v.start = window > 0 ? max(0, v.length - window) : 0;
+  const int end = (v.length + kCachePage - 1) / kCachePage;
+  v.back = v.start / kCachePage;
+  v.front = v.start > 0 ? min((first + kCachePage - 1) / kCachePage, v.back) : 0;
+  v.pages = v.front + end - v.back;
+  return v;
+}
+
+// NT: tiles of 8 query heads of one kv head that share the loaded codes.
+template <typename T, int D, int NT, int CP>
+__global__ void __launch_bounds__(kWarps * 32)
+row_kernel(const AttentionParams p) {
+  constexpr int KW = D / 16;   // 32-bit words of keys a lane holds for each of its two tokens
+  constexpr int VW = D / 32;   // words of values a lane holds for each of its four tokens
+  constexpr int kStride = D + 2;
+  const int split = blockIdx.x % p.splits;
+  const int row = blockIdx.x / p.splits;
+  const int kv_head = blockIdx.y / p.head_tiles;
+  const int head_base = (blockIdx.y % p.head_tiles) * (8 * NT);  // within the group
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, c = lane & 3;
+  __shared__ float merged[kWarps][8 * NT][kStride];
+
+  const int sequence =
+      p.offsets == nullptr ? row : sequence_of_row(p.offsets, p.cache.batch, row);
+  if (sequence < 0) return;  // a row of no sequence is left as it was
+  int length = sequence_length(p.cache, sequence, p.status);
+  if (p.offsets != nullptr) length += row + 1 - p.offsets[sequence + 1];
+  const Visible v = visible_pages(length, p.window, p.first);
+  const int per_split = (v.pages + p.splits - 1) / p.splits;
+  const int page_begin = split * per_split;
+  const int page_end = min(v.pages, page_begin + per_split);
+
+  // Queries as B fragments: head g of every tile, the dimensions that this lane's key words hold
+  // (word w of a token: dimensions 64 (w / 4) + 16 c + 4 (w % 4) .. + 3).
+  uint32_t q[NT][KW][2];
+  float factor[NT][2];  // scale * log2(e) / (the row's power of two) of heads 2c and 2c + 1
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int head = head_base + 8 * n + g;
+    const bool live = head < p.group;
+    const T* source = static_cast<const T*>(p.query) + static_cast<int64_t>(row) * p.query_token_stride +
+                      (kv_head * p.group + head) * p.query_head_stride + 16 * c;
+    uint32_t words[KW][2];
+#pragma unroll
+    for (int w = 0; w < KW; w += 4) {
+      uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+      if (live) {
+        lo = *reinterpret_cast<const uint4*>(source + 64 * (w / 4));
+        hi = *reinterpret_cast<const uint4*>(source + 64 * (w / 4) + 8);
+      }
+      words[w][0] = lo.x; words[w][1] = lo.y; words[w + 1][0] = lo.z; words[w + 1][1] = lo.w;
+      words[w + 2][0] = hi.x; words[w + 2][1] = hi.y; words[w + 3][0] = hi.z;
+      words[w + 3][1] = hi.w;
+    }
+    float inverse = 1.0f;
+    if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        q[n][w][0] = words[w][0];
+        q[n][w][1] = words[w][1];
+      }
+    } else {
+      uint32_t largest = 0;
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          largest = max(largest, max((words[w][i] & 0x7fffu) << 16, words[w][i] & 0x7fff0000u));
+        }
+      }
+      largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+      largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+      // power of two that puts the row's largest into [2^14, 2^15); none for zeros, NaN, infinity
+      int shift = 14 - (static_cast<int>(largest >> 23) - 127);
+      shift = largest == 0 || largest >= 0x7f800000u ? 0 : min(shift, 100);
+      const float up = exp2_int(shift);
+      inverse = exp2_int(-shift);
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          q[n][w][i] = Elem<__half>::pack2(Elem<T>::from_bits(words[w][i] & 0xffffu) * up,
+                                           Elem<T>::from_bits(words[w][i] >> 16) * up);
+        }
+      }
+    }
+    factor[n][0] = p.scale_log2 * __shfl_sync(0xffffffffu, inverse, 8 * c);
+    factor[n][1] = p.scale_log2 * __shfl_sync(0xffffffffu, inverse, 8 * c + 4);
+  }
+
+  float running_max[NT][2], running_sum[NT][2];
+  float out[NT][2 * VW][4];  // tile i: dimensions D/8 g + 2i (registers 0, 1) and + 1 (2, 3)
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    running_max[n][0] = running_max[n][1] = -INFINITY;
+    running_sum[n][0] = running_sum[n][1] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2 * VW; ++i) out[n][i][0] = out[n][i][1] = out[n][i][2] = out[n][i][3] = 0;
+  }
+
+  // Codes of a chunk: keys of tokens g and g + 8, values of tokens 2c, 2c+1, 2c+8, 2c+9.
+  uint32_t keys[CP][2][KW], values[CP][4][VW];
+  // lane i holds block index and scale bytes of page i of the chunk
+  int64_t block = -1;
+  uint32_t key_byte = 0, value_byte = 0;
+  auto look_up = [&](int index) {
+    block = -1;
+    key_byte = value_byte = 127;
+    if (lane < CP && index + lane < page_end) {
+      const int i = index + lane;
+      const int page = physical_page(p.cache, sequence, i < v.front ? i : i - v.front + v.back,
+                                     p.status);
+      if (page >= 0) {
+        block = static_cast<int64_t>(page) * p.cache.kv_heads + kv_head;
+        key_byte = p.cache.scales[0][block];
+        value_byte = p.cache.scales[1][block];
+      }
+    }
+  };
+  auto load_keys = [&]() {
+#pragma unroll
+    for (int i = 0; i < CP; ++i) {
+      const int64_t b = __shfl_sync(0xffffffffu, block, i);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int w = 0; w < KW; w += 4) {
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (b >= 0) {
+            x = *reinterpret_cast<const uint4*>(p.cache.codes[0] + b * (kCachePage * D) +
+                                                (g + 8 * h) * D + 64 * (w / 4) + 16 * c);
+          }
+          keys[i][h][w] = x.x; keys[i][h][w + 1] = x.y;
+          keys[i][h][w + 2] = x.z; keys[i][h][w + 3] = x.w;
+        }
+      }
+    }
+  };
+  auto load_values = [&]() {
+#pragma unroll
+    for (int i = 0; i < CP; ++i) {
+      const int64_t b = __shfl_sync(0xffffffffu, block, i);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const uint8_t* source = p.cache.codes[1] + b * (kCachePage * D) +
+                                (2 * c + (t & 1) + 8 * (t >> 1)) * D + (D / 8) * g;
+        if constexpr (VW == 2) {
+          uint2 x = make_uint2(0, 0);
+          if (b >= 0) x = *reinterpret_cast<const uint2*>(source);
+          values[i][t][0] = x.x; values[i][t][1] = x.y;
+        } else {
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (b >= 0) x = *reinterpret_cast<const uint4*>(source);
+          values[i][t][0] = x.x; values[i][t][1] = x.y;
+          values[i][t][2] = x.z; values[i][t][3] = x.w;
+        }
+      }
+    }
+  };
+
+  int index = page_begin + warp * CP;
+  if (index < page_end) {
+    look_up(index);
+    load_keys();
+    load_values();
+  }
+  for (; index < page_end; index += kWarps * CP) {
+    // visibility of this chunk's pages, then the next chunk's table entries
+    bool present[CP];
+    float key_scale[CP], value_exponent[CP];
+#pragma unroll
+    for (int i = 0; i < CP; ++i) {
+      present[i] = __shfl_sync(0xffffffffu, block, i) >= 0;
+      key_scale[i] = exp2_int(scale_exponent(__shfl_sync(0xffffffffu, key_byte, i)));
+      value_exponent[i] =
+          static_cast<float>(scale_exponent(__shfl_sync(0xffffffffu, value_byte, i)));
+    }
+    look_up(index + kWarps * CP);
+
+    float s[NT][CP][4];  // tokens g (0, 1) and g + 8 (2, 3), heads 2c and 2c + 1
+#pragma unroll
+    for (int i = 0; i < CP; ++i) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n][i][0] = s[n][i][1] = s[n][i][2] = s[n][i][3] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        const uint32_t a0 = e4m3x2_to_f16x2(keys[i][0][w] & 0xffffu);
+        const uint32_t a2 = e4m3x2_to_f16x2(keys[i][0][w] >> 16);
+        const uint32_t a1 = e4m3x2_to_f16x2(keys[i][1][w] & 0xffffu);
+        const uint32_t a3 = e4m3x2_to_f16x2(keys[i][1][w] >> 16);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_f16(s[n][i], a0, a1, a2, a3, q[n][w][0], q[n][w][1]);
+      }
+    }
+    if (index + kWarps * CP < page_end) load_keys();
+
+    // scores into the exponent's domain; a page's tokens are masked only where some are unseen
+    float chunk_max[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) chunk_max[n][0] = chunk_max[n][1] = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < CP; ++i) {
+      const int logical = index + i < v.front ? index + i : index + i - v.front + v.back;
+      const int token = logical * kCachePage;
+      const bool whole = present[i] && token + kCachePage <= v.length &&
+                         (token >= v.start || token + kCachePage <= p.first);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][i][j] *= factor[n][j & 1] * key_scale[i];
+      }
+      if (!whole) {
+        auto seen = [&](int t) {
+          return present[i] && t < v.length && (t >= v.start || t < p.first);
+        };
+        const bool seen_g = seen(token + g), seen_h = seen(token + g + 8);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          if (!seen_g) s[n][i][0] = s[n][i][1] = -INFINITY;
+          if (!seen_h) s[n][i][2] = s[n][i][3] = -INFINITY;
+        }
+        // whatever an unseen slot holds must not meet the product: 0 * NaN
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          if (!seen(token + 2 * c + (t & 1) + 8 * (t >> 1))) {
+#pragma unroll
+            for (int w = 0; w < VW; ++w) values[i][t][w] = 0;
+          }
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        chunk_max[n][0] = fmaxf(chunk_max[n][0],
+                                fmaxf(s[n][i][0], s[n][i][2]) + value_exponent[i]);
+        chunk_max[n][1] = fmaxf(chunk_max[n][1],
+                                fmaxf(s[n][i][1], s[n][i][3]) + value_exponent[i]);
+      }
+    }
+    float base[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float m = chunk_max[n][j];
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+        m = fmaxf(m, running_max[n][j]);
+        // nothing seen yet: leave the (empty) state as it is
+        const float rescale = m == -INFINITY ? 1.0f : exp2f(running_max[n][j] - m);
+        base[n][j] = m == -INFINITY ? 0.0f : m;
+        running_max[n][j] = m;
+        running_sum[n][j] *= rescale;
+#pragma unroll
+        for (int i = 0; i < 2 * VW; ++i) {
+          out[n][i][j] *= rescale;
+          out[n][i][j + 2] *= rescale;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < CP; ++i) {
+      const float unscale = exp2f(-value_exponent[i]);
+      uint32_t weights[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float w0 = exp2f(s[n][i][0] + (value_exponent[i] - base[n][0]));
+        const float w1 = exp2f(s[n][i][1] + (value_exponent[i] - base[n][1]));
+        const float w2 = exp2f(s[n][i][2] + (value_exponent[i] - base[n][0]));
+        const float w3 = exp2f(s[n][i][3] + (value_exponent[i] - base[n][1]));
+        running_sum[n][0] = fmaf(w0 + w2, unscale, running_sum[n][0]);
+        running_sum[n][1] = fmaf(w1 + w3, unscale, running_sum[n][1]);
+        weights[n][0] = transpose8x8(Elem<__half>::pack2(w0, w1));
+        weights[n][1] = transpose8x8(Elem<__half>::pack2(w2, w3));
+      }
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+        const uint32_t lo01 = __byte_perm(values[i][0][w], values[i][1][w], 0x5140);
+        const uint32_t lo23 = __byte_perm(values[i][0][w], values[i][1][w], 0x7362);
+        const uint32_t hi01 = __byte_perm(values[i][2][w], values[i][3][w], 0x5140);
+        const uint32_t hi23 = __byte_perm(values[i][2][w], values[i][3][w], 0x7362);
+        const uint32_t a[2][4] = {
+            {e4m3x2_to_f16x2(lo01 & 0xffffu), e4m3x2_to_f16x2(lo01 >> 16),
+             e4m3x2_to_f16x2(hi01 & 0xffffu), e4m3x2_to_f16x2(hi01 >> 16)},
+            {e4m3x2_to_f16x2(lo23 & 0xffffu), e4m3x2_to_f16x2(lo23 >> 16),
+             e4m3x2_to_f16x2(hi23 & 0xffffu), e4m3x2_to_f16x2(hi23 >> 16)}};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            mma_f16(out[n][2 * w + h], a[h][0], a[h][1], a[h][2], a[h][3], weights[n][0],
+                    weights[n][1]);
+          }
+        }
+      }
+    }
+    if (index + kWarps * CP < page_end) load_values();
+  }
+
+  // ---- merge the warps ----
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float sum = running_sum[n][j];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+      float* state = merged[warp][8 * n + 2 * c + j];
+#pragma unroll
+      for (int i = 0; i < 2 * VW; ++i) {
+        state[(D / 8) * g + 2 * i] = out[n][i][j];
+        state[(D / 8) * g + 2 * i + 1] = out[n][i][j + 2];
+      }
+      if (g == 0) {
+        state[D] = running_max[n][j];
+        state[D + 1] = sum;
+      }
+    }
+  }
+  __syncthreads();
+  for (int item = threadIdx.x; item < 8 * NT * (D / 4); item += kWarps * 32) {
+    const int h = item / (D / 4), d0 = 4 * (item % (D / 4));
+    const int head = head_base + h;
+    if (head >= p.group) continue;
+    float total_max = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) total_max = fmaxf(total_max, merged[w][h][D]);
+    float total_sum = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float m = merged[w][h][D];
+      const float weight = m == -INFINITY ? 0.0f : exp2f(m - total_max);
+      total_sum += merged[w][h][D + 1] * weight;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = fmaf(merged[w][h][d0 + i], weight, acc[i]);
+    }
+    const int64_t query_head = static_cast<int64_t>(row) * p.query_heads + kv_head * p.group + head;
+    if (p.splits > 1) {
+      float* destination = p.partial + (query_head * p.splits + split) * kStride;
+      *reinterpret_cast<float2*>(destination + d0) = make_float2(acc[0], acc[1]);
+      *reinterpret_cast<float2*>(destination + d0 + 2) = make_float2(acc[2], acc[3]);
+      if (d0 == 0) {
+        *reinterpret_cast<float2*>(destination + D) = make_float2(total_max, total_sum);
+      }
+    } else {
+      float denominator = total_sum;
+      if (p.sinks != nullptr) {
+        denominator += exp2f(p.sinks[kv_head * p.group + head] * kLog2e - total_max);
+      }
+      // only a row that sees nothing has a sum of exactly zero; its output is zero
+      const float inverse = total_sum == 0.0f ? 0.0f : 1.0f / denominator;
+      T* out_row = static_cast<T*>(p.output) + query_head * D + d0;
+      *reinterpret_cast<uint2*>(out_row) =
+          make_uint2(Elem<T>::pack2(acc[0] * inverse, acc[1] * inverse),
+                     Elem<T>::pack2(acc[2] * inverse, acc[3] * inverse));
+    }
+  }
+}
+
+// One warp per query head of a row: joins the splits, applies the sink, narrows.
+template <typename T, int D>
+__global__ void __launch_bounds__(128)
+join_kernel(const AttentionParams p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t query_head = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (query_head >= static_cast<int64_t>(p.tokens) * p.query_heads) return;
+  const int row = static_cast<int>(query_head / p.query_heads);
+  if (p.offsets != nullptr && sequence_of_row(p.offsets, p.cache.batch, row) < 0) return;
+  const float* base = p.partial + query_head * p.splits * (D + 2);
+  float total_max = -INFINITY;
+  for (int s = 0; s < p.splits; ++s) total_max = fmaxf(total_max, base[s * (D + 2) + D]);
+  float total_sum = 0.0f, acc[D / 32] = {};
+  for (int s = 0; s < p.splits; ++s) {
+    const float* part = base + s * (D + 2);
+    const float m = part[D];
+    const float weight = m == -INFINITY ? 0.0f : exp2f(m - total_max);
+    total_sum += part[D + 1] * weight;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      const float2 x = *reinterpret_cast<const float2*>(part + 64 * i + 2 * lane);
+      acc[2 * i] = fmaf(x.x, weight, acc[2 * i]);
+      acc[2 * i + 1] = fmaf(x.y, weight, acc[2 * i + 1]);
+    }
+  }
+  float denominator = total_sum;
+  if (p.sinks != nullptr) {
+    denominator += exp2f(p.sinks[query_head % p.query_heads] * kLog2e - total_max);
+  }
+  const float inverse = total_sum == 0.0f ? 0.0f : 1.0f / denominator;
+  T* out = static_cast<T*>(p.output) + query_head * D + 2 * lane;
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) {
+    *reinterpret_cast<uint32_t*>(out + 64 * i) =
+        Elem<T>::pack2(acc[2 * i] * inverse, acc[2 * i + 1] * inverse);
+  }
+}
+
+template <typename T, int D>
+void launch_rows(const AttentionParams& p, cudaStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(p.tokens) * p.splits),
+                  static_cast<unsigned>(p.cache.kv_heads * p.head_tiles));
+  if (p.group <= 8) {
+    row_kernel<T, D, 1, 256 / D><<<grid, kWarps * 32, 0, stream>>>(p);
+  } else {
+    row_kernel<T, D, 2, 128 / D><<<grid, kWarps * 32, 0, stream>>>(p);
+  }
+  if (p.splits > 1) {
+    const int64_t heads = static_cast<int64_t>(p.tokens) * p.query_heads;
+    join_kernel<T, D><<<static_cast<unsigned>((heads + 3) / 4), 128, 0, stream>>>(p);
+  }
+}
+
+// Pages that a row can see at most.
+int64_t most_pages(const NmlSm100PagedAttentionQ8& r) {
+  if (r.sliding_window == 0) return r.cache.table_width;
+  const int64_t pages = (r.sliding_window + kCachePage - 1) / kCachePage + 1 +
+                        (r.first_tokens + kCachePage - 1) / kCachePage;
+  return pages < r.cache.table_width ? pages : r.cache.table_width;
+}
+
+// Splits of the visible pages: until there are two CTAs for every SM, at least eight pages each.
+int64_t choose_splits(const NmlSm100PagedAttentionQ8& r) {
+  if (r.splits > 0) return r.splits;
+  constexpr int64_t kWanted = 2 * 148;
+  const int64_t pairs = r.tokens * r.cache.kv_heads;
+  int64_t splits = (kWanted + pairs - 1) / pairs;
+  const int64_t most = most_pages(r) / 8;
+  if (splits > most) splits = most;
+  return splits < 1 ? 1 : splits > 64 ? 64 : splits;
+}
+
+bool valid_request(const NmlSm100PagedAttentionQ8& r) {
+  return fits_i32(r.tokens) && r.cache.kv_heads > 0 && r.query_heads > 0 &&
+         r.query_heads % r.cache.kv_heads == 0 && r.query_heads / r.cache.kv_heads <= 128 &&
+         (r.cache.head_dim == 64 || r.cache.head_dim == 128) && fits_i32(r.cache.batch) &&
+         fits_i32(r.cache.table_width) && r.splits >= 0 && r.splits <= 64 &&
+         r.sliding_window >= 0 && r.first_tokens >= 0 &&
+         r.sliding_window <= std::numeric_limits<int32_t>::max() &&
+         r.first_tokens <= std::numeric_limits<int32_t>::max() - kCachePage;
+}
+
+}  // namespace
+}  // namespace nml_sm100
+
+using namespace nml_sm100;
+
+extern "C" size_t nml_sm100_paged_attention_q8_workspace_bytes(
+    const NmlSm100PagedAttentionQ8* request) {
+  if (request == nullptr || request->struct_size < sizeof(NmlSm100PagedAttentionQ8) ||
+      !valid_request(*request)) {
+    return 0;
+  }
+  const int64_t splits = choose_splits(*request);
+  if (splits <= 1) return 0;
+  return static_cast<size_t>(request->tokens) * request->query_heads * splits *
+         (request->cache.head_dim + 2) * sizeof(float);
+}
+
+extern "C" int32_t nml_sm100_paged_attention_q8(const NmlSm100PagedAttentionQ8* request,
+                                                char* error_message,
+                                                size_t error_message_capacity) {
+  if (request == nullptr || request->struct_size < sizeof(NmlSm100PagedAttentionQ8)) {
+    return fail(NML_SM100_INVALID_ARGUMENT, "truncated paged attention request", error_message,
+                error_message_capacity);
+  }
+  const NmlSm100PagedAttentionQ8& r = *request;
+  if (!valid_cache_q8(r.cache, true) || !valid_request(r) || r.query == nullptr ||
+      r.output == nullptr || r.stream == nullptr ||
+      (r.query_offsets == nullptr && r.tokens != r.cache.batch) ||
+      r.query_token_stride % 8 != 0 || r.query_head_stride % 8 != 0 ||
+      r.query_token_stride < 0 || r.query_head_stride < 0 ||
+      r.cache.kv_heads > 1024 || !(r.scale > 0.0f) ||
+      r.scale > std::numeric_limits<float>::max() ||
+      reinterpret_cast<uintptr_t>(r.query) % 16 != 0 ||
+      reinterpret_cast<uintptr_t>(r.output) % 16 != 0 ||
+      reinterpret_cast<uintptr_t>(r.workspace) % 16 != 0) {
+    return fail(NML_SM100_INVALID_ARGUMENT,
+                "invalid 8-bit paged attention request (head_dim 64 or 128, page size 16, at most "
+                "128 query heads per kv head)",
+                error_message, error_message_capacity);
+  }
+  if (r.dtype != NML_SM100_F16 && r.dtype != NML_SM100_BF16) {
+    return fail(NML_SM100_INVALID_ARGUMENT, "paged attention supports F16 and BF16 only",
+                error_message, error_message_capacity);
+  }
+  const int64_t splits = choose_splits(r);
+  if (r.tokens * splits > std::numeric_limits<int32_t>::max()) {
+    return fail(NML_SM100_INVALID_ARGUMENT, "invalid 8-bit paged attention request: too many rows",
+                error_message, error_message_capacity);
+  }
+  const size_t needed = nml_sm100_paged_attention_q8_workspace_bytes(request);
+  if (needed > 0 && (r.workspace == nullptr || r.workspace_bytes < needed)) {
+    return fail(NML_SM100_INVALID_ARGUMENT, "paged attention workspace is too small",
+                error_message, error_message_capacity);
+  }
+  const DeviceInfo* device = current_device(error_message, error_message_capacity);
+  if (device == nullptr) return NML_SM100_LAUNCH_FAILURE;
+  AttentionParams p = {};
+  p.cache = cache_params(r.cache);
+  p.query = r.query;
+  p.offsets = r.query_offsets;
+  p.sinks = r.sinks;
+  p.partial = static_cast<float*>(r.workspace);
+  p.output = r.output;
+  p.query_token_stride = r.query_token_stride;
+  p.query_head_stride = r.query_head_stride;
+  p.tokens = static_cast<int>(r.tokens);
+  p.query_heads = static_cast<int>(r.query_heads);
+  p.group = static_cast<int>(r.query_heads / r.cache.kv_heads);
+  p.head_tiles = p.group <= 8 ? 1 : (p.group + 15) / 16;
+  p.splits = static_cast<int>(splits);
+  p.window = static_cast<int>(r.sliding_window);
+  p.first = static_cast<int>(r.first_tokens);
+  p.scale_log2 = r.scale * kLog2e;
+  p.status = device->status_word;
+  cudaStream_t stream = static_cast<cudaStream_t>(r.stream);
+  const bool half = r.dtype == NML_SM100_F16;
+  if (r.cache.head_dim == 64) {
+    half ? launch_rows<__half, 64>(p, stream) : launch_rows<__nv_bfloat16, 64>(p, stream);
+  } else {
+    half ? launch_rows<__half, 128>(p, stream) : launch_rows<__nv_bfloat16, 128>(p, stream);
+  }
+  return launch_result(error_message, error_message_capacity);
+}

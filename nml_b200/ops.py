@@ -545,6 +545,233 @@ def paged_attention_decode(query: torch.Tensor, key_cache: torch.Tensor,
     return out
 
 
+# ------------------------------------------------------------------ 8-bit paged K/V cache
+
+def rotary_table(frequencies: torch.Tensor, positions: int,
+                 attention_factor: float = 1.0) -> torch.Tensor:
+    """f32 [positions, 2 * len(frequencies)] table of ``paged_append_q8``: cosines, then sines, of
+    every position times every inverse frequency, both times ``attention_factor`` (the factor a
+    model scales long contexts with, 1 without).  The angles are formed in 64 bits: far positions
+    lose none of their phase."""
+    if frequencies.dim() != 1 or frequencies.numel() == 0 or positions <= 0:
+        raise ValueError("rotary table expects a vector of frequencies and a positive extent")
+    index = torch.arange(positions, dtype=torch.float64, device=frequencies.device)
+    angles = index[:, None] * frequencies.double()
+    return (torch.cat((angles.cos(), angles.sin()), dim=1) * attention_factor).float()
+
+
+def _call_on(device: torch.device, name: str, request) -> None:
+    """The library launches on the current device; make that the tensors' own."""
+    if device.index == torch.cuda.current_device():
+        _abi.call(name, request)
+    else:
+        with torch.cuda.device(device):
+            _abi.call(name, request)
+
+
+def _cache_q8(key_cache, key_scales, value_cache, value_scales, page_table, sequence_lengths,
+              device) -> _abi.CacheQ8:
+    shape = key_cache.shape
+    if len(shape) != 4 or value_cache.shape != shape or key_scales.shape != shape[:2] or \
+            value_scales.shape != shape[:2]:
+        raise ValueError("8-bit caches are codes [pages, kv_heads, page_size, head_dim] and scales "
+                         "[pages, kv_heads], keys and values alike")
+    pages, kv_heads, page_size, head_dim = shape
+    batch = page_table.shape[0] if page_table.dim() == 2 else -1
+    if page_table.dtype != torch.int32 or batch < 0 or (
+            sequence_lengths is not None and (sequence_lengths.dtype != torch.int32 or
+                                              sequence_lengths.shape != (batch,))):
+        raise ValueError("page table must be I32 [batch, pages], sequence lengths I32 [batch]")
+    for tensor in (key_cache, key_scales, value_cache, value_scales):
+        if tensor.dtype != torch.uint8:
+            raise ValueError("8-bit caches and their scales must use U8 buffers")
+    for tensor in (key_cache, key_scales, value_cache, value_scales, page_table,
+                   sequence_lengths):
+        if tensor is None:
+            continue
+        if not tensor.is_contiguous():
+            raise ValueError("8-bit caches, page tables and lengths must be contiguous")
+        if tensor.device != device:
+            raise ValueError("the tensors of a call must live on one CUDA device")
+    return _abi.CacheQ8(key_cache.data_ptr(), key_scales.data_ptr(), value_cache.data_ptr(),
+                        value_scales.data_ptr(), page_table.data_ptr(), _ptr(sequence_lengths),
+                        batch, kv_heads, head_dim, page_size, pages, page_table.shape[1])
+
+
+def _head_rows(tensor: torch.Tensor, what: str, tokens: int, heads: int, dim: int, dtype, device):
+    """Strides (in elements) of [tokens, heads, dim] rows; views into a wider row (the fused
+    projection's output) are fine, the elements of one head lie together."""
+    if tensor.shape != (tokens, heads, dim) or tensor.dtype != dtype:
+        raise ValueError(f"{what} must be [tokens, heads, head_dim] rows of the call's dtype")
+    if tensor.device != device:
+        raise ValueError("the tensors of a call must live on one CUDA device")
+    token, head, element = tensor.stride()
+    # the stride of an extent of one is never used
+    token, head = token if tokens > 1 else 0, head if heads > 1 else 0
+    if element != 1 or token % 8 != 0 or head % 8 != 0 or tensor.data_ptr() % 16 != 0:
+        raise ValueError(f"{what}: heads must be contiguous, rows and heads 16-byte aligned")
+    return token, head
+
+
+def _row_offsets(offsets, batch: int, tokens: int, device) -> None:
+    if offsets is None:
+        if tokens != batch:
+            raise ValueError("without offsets every sequence has exactly one row")
+    elif offsets.dtype != torch.int32 or offsets.shape != (batch + 1,) or \
+            not offsets.is_contiguous() or offsets.device != device:
+        raise ValueError("row offsets must be I32 [batch + 1] on the call's device")
+
+
+def _require_device(tensor: torch.Tensor) -> torch.device:
+    if not tensor.is_cuda:
+        raise RuntimeError("8-bit cache operators run on a CUDA device only (no CPU fallback)")
+    return tensor.device
+
+
+def paged_append_q8(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
+                    key_scales: torch.Tensor, value_cache: torch.Tensor,
+                    value_scales: torch.Tensor, page_table: torch.Tensor,
+                    sequence_lengths: torch.Tensor, token_offsets: torch.Tensor | None = None,
+                    query: torch.Tensor | None = None, rotary: torch.Tensor | None = None,
+                    rotary_layout: str = "half") -> torch.Tensor | None:
+    """Rotates keys (and ``query``), quantises keys and values and writes them into the 8-bit
+    paged cache, in one launch; returns the rotated query (``None`` without one).
+
+    ``key``, ``value`` [tokens, kv_heads, head_dim] and ``query`` [tokens, query_heads, head_dim]
+    are the last tokens of their sequences, rows ``token_offsets[b] .. token_offsets[b + 1]`` of
+    sequence b (I32 [batch + 1]; ``None``: one row each); views of a fused projection's rows are
+    fine.  ``sequence_lengths`` counts them in, 0 for an empty place of a padded batch, whose
+    query row becomes zero.  The caches (changed in place) are codes U8 [pages, kv_heads, 16,
+    head_dim] and block scales U8 [pages, kv_heads] as ``nml_sm100_paged_append_q8`` describes
+    them; a written page belongs to one sequence.  ``rotary`` is the table of ``rotary_table``
+    (its width is the rotated part of the head), ``rotary_layout`` pairs elements of the two
+    halves (``"half"``) or neighbours (``"interleaved"``)."""
+    device = _require_device(key)
+    if key.dim() != 3:
+        raise ValueError("keys must be [tokens, kv_heads, head_dim]")
+    if rotary_layout not in ("half", "interleaved"):
+        raise ValueError("rotary layout must be 'half' or 'interleaved'")
+    cache = _cache_q8(key_cache, key_scales, value_cache, value_scales, page_table,
+                      sequence_lengths, device)
+    tokens, kv_heads, dim = key.shape
+    if kv_heads != cache.kv_heads or dim != cache.head_dim:
+        raise ValueError("key and cache head geometry is incompatible")
+    dtype = _code(key.dtype)
+    _row_offsets(token_offsets, cache.batch, tokens, device)
+    key_strides = _head_rows(key, "keys", tokens, kv_heads, dim, key.dtype, device)
+    value_strides = _head_rows(value, "values", tokens, kv_heads, dim, key.dtype, device)
+    rotated, heads, query_strides = None, 0, (0, 0)
+    if query is not None:
+        if query.dim() != 3:
+            raise ValueError("queries must be [tokens, query_heads, head_dim]")
+        heads = query.shape[1]
+        query_strides = _head_rows(query, "queries", tokens, heads, dim, key.dtype, device)
+    if rotary is not None and (rotary.dim() != 2 or rotary.dtype != torch.float32 or
+                               not rotary.is_contiguous() or rotary.device != device):
+        raise ValueError("the rotary table must be F32 [positions, width] on the call's device")
+    if tokens == 0:
+        return None if query is None else torch.empty_like(query)
+    if query is not None:
+        rotated = torch.empty((tokens, heads, dim), dtype=query.dtype, device=device)
+    rotary_rows, rotary_dim = (0, 0) if rotary is None else rotary.shape
+    request = _abi.PagedAppendQ8(
+        0, cache, key.data_ptr(), value.data_ptr(), _ptr(query), _ptr(rotated),
+        _ptr(token_offsets), _ptr(rotary), _stream(key), tokens, heads, *key_strides,
+        *value_strides, *query_strides, heads * dim, dim, rotary_rows, rotary_dim,
+        1 if rotary_layout == "interleaved" else 0, dtype)
+    _call_on(device, "nml_sm100_paged_append_q8", request)
+    return rotated
+
+
+def paged_read_q8(key_cache: torch.Tensor, key_scales: torch.Tensor, value_cache: torch.Tensor,
+                  value_scales: torch.Tensor, page_table: torch.Tensor,
+                  token_offsets: torch.Tensor, tokens: int,
+                  dtype: torch.dtype = torch.bfloat16, out=None):
+    """Reads tokens back from the 8-bit paged cache: rows ``token_offsets[b] ..
+    token_offsets[b + 1]`` of the two results [tokens, kv_heads, head_dim] are the first tokens of
+    sequence b.  ``tokens`` is the results' row count; rows outside every sequence are left as
+    they were (``out``: a pair of contiguous tensors to write into)."""
+    device = _require_device(key_cache)
+    cache = _cache_q8(key_cache, key_scales, value_cache, value_scales, page_table, None, device)
+    if token_offsets is None:
+        raise ValueError("reading back needs the sequences' row offsets")
+    _row_offsets(token_offsets, cache.batch, tokens, device)
+    code = _code(dtype)
+    shape = (tokens, cache.kv_heads, cache.head_dim)
+    if tokens < 0:
+        raise ValueError("the row count must not be negative")
+    if out is None:
+        out = (torch.empty(shape, dtype=dtype, device=device),
+               torch.empty(shape, dtype=dtype, device=device))
+    else:
+        for tensor in out:
+            if tensor.shape != shape or tensor.dtype != dtype or tensor.device != device or \
+                    not tensor.is_contiguous():
+                raise ValueError("read-back outputs must be contiguous [tokens, kv_heads, "
+                                 "head_dim] of the call's dtype and device")
+    if tokens == 0:
+        return out
+    request = _abi.PagedReadQ8(0, cache, token_offsets.data_ptr(), out[0].data_ptr(),
+                               out[1].data_ptr(), _stream(key_cache), tokens, code)
+    _call_on(device, "nml_sm100_paged_read_q8", request)
+    return out
+
+
+def paged_attention_q8(query: torch.Tensor, key_cache: torch.Tensor, key_scales: torch.Tensor,
+                       value_cache: torch.Tensor, value_scales: torch.Tensor,
+                       page_table: torch.Tensor, sequence_lengths: torch.Tensor,
+                       query_offsets: torch.Tensor | None = None,
+                       sinks: torch.Tensor | None = None, sliding_window: int | None = None,
+                       first_tokens: int = 0, scale: float | None = None,
+                       splits: int | None = None,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention over the 8-bit paged cache: the operator of ``paged_attention_decode``
+    for caches that ``paged_append_q8`` writes, for single tokens and for runs of them.
+
+    ``query`` [tokens, query_heads, head_dim] are the last tokens of their sequences: rows
+    ``query_offsets[b] .. query_offsets[b + 1]`` of sequence b, or one row each (``None``).
+    Every query sees the tokens up to its own; with ``sliding_window`` only the last that many of
+    them, and the first ``first_tokens`` of the sequence.  ``sinks`` F32 [query_heads] adds a
+    column without a value to the softmax.  A row that sees nothing (an empty place of a padded
+    batch) becomes zeros; rows outside every sequence are left as they were in ``out``.  Scratch
+    is allocated per call from torch's allocator, so captured graphs never share it."""
+    device = _require_device(query)
+    if query.dim() != 3:
+        raise ValueError("paged attention expects query [tokens, heads, dim]")
+    cache = _cache_q8(key_cache, key_scales, value_cache, value_scales, page_table,
+                      sequence_lengths, device)
+    tokens, heads, dim = query.shape
+    if dim != cache.head_dim or cache.kv_heads == 0 or heads % cache.kv_heads != 0:
+        raise ValueError("paged query/KV head geometry is incompatible")
+    code = _code(query.dtype)
+    _row_offsets(query_offsets, cache.batch, tokens, device)
+    strides = _head_rows(query, "queries", tokens, heads, dim, query.dtype, device)
+    if sinks is not None and (sinks.dtype != torch.float32 or sinks.shape != (heads,) or
+                              not sinks.is_contiguous() or sinks.device != device):
+        raise ValueError("attention sinks must be F32 [query_heads]")
+    if (sliding_window is not None and sliding_window <= 0) or first_tokens < 0 or \
+            (splits is not None and splits <= 0):
+        raise ValueError("window and splits must be positive, first tokens not negative")
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=query.dtype, device=device)
+    elif out.shape != query.shape or out.dtype != query.dtype or out.device != device or \
+            not out.is_contiguous():
+        raise ValueError("the attention output must be contiguous, of the query's shape and dtype")
+    if tokens == 0:
+        return out
+    request = _abi.PagedAttentionQ8(
+        0, cache, query.data_ptr(), _ptr(query_offsets), _ptr(sinks), out.data_ptr(), None, 0,
+        _stream(query), tokens, heads, *strides, sliding_window or 0, first_tokens, splits or 0,
+        dim ** -0.5 if scale is None else scale, code)
+    request.struct_size = ctypes.sizeof(request)
+    size = _abi.load().nml_sm100_paged_attention_q8_workspace_bytes(ctypes.byref(request))
+    if size:
+        scratch = torch.empty(size, dtype=torch.uint8, device=device)
+        request.workspace, request.workspace_bytes = scratch.data_ptr(), size
+    _call_on(device, "nml_sm100_paged_attention_q8", request)
+    return out
+
+
 def topk_rows(logits: torch.Tensor, k: int, index_offset: int = 0):
     """(values f32 [rows, k], indices i32 [rows, k]) of the k largest entries of every row of a
     16-bit matrix, descending, equal values to the lower index (``nml_nvfp4_sm100_topk_rows``)."""

@@ -1,0 +1,290 @@
+"""Attention over the 8-bit paged cache against its definition in 64 bits over the same codes.
+The tolerance is derived in cache_q8_reference.attention from the roundings that the operator
+documents; it scales with the weights' own magnitudes, not with the output's."""
+import pytest
+import torch
+
+import cache_q8_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def status():
+    from nml_b200 import _abi
+    torch.cuda.synchronize()
+    return _abi.device_status(0x1)
+
+
+def make(seed, dtype, dim, kv_heads, group, new, before, spread=0.0, with_sinks=False):
+    gen = torch.Generator().manual_seed(seed)
+    lengths = [n + m if m is not None else 0 for n, m in zip(new, before)]
+    table, pages = ref.random_table(gen, lengths)
+    cache = ref.stale(ref.random_cache(gen, pages, kv_heads, dim, spread), table, lengths, gen)
+    query = torch.randn((sum(new), kv_heads * group, dim), generator=gen).to(dtype)
+    sinks = torch.randn(kv_heads * group, generator=gen) if with_sinks else None
+    return lengths, table, cache, query, sinks, ref.offsets_of(new)
+
+
+def call(query, cache, table, lengths, offsets, sinks, **options):
+    from nml_b200 import ops
+    return ops.paged_attention_q8(
+        query.cuda(), *[x.cuda() for x in cache], table.cuda(),
+        torch.tensor(lengths, dtype=torch.int32).cuda(),
+        query_offsets=None if offsets is None else torch.tensor(offsets, dtype=torch.int32).cuda(),
+        sinks=None if sinks is None else sinks.cuda(), **options)
+
+
+SINGLE = [
+    # dim, kv_heads, group, tokens before each query (None: an empty place), window, first, sinks
+    (64, 8, 8, [0, 15, 16, 4095], 0, 0, True),
+    (64, 2, 8, [99, None, 700, None], 0, 0, True),
+    (64, 1, 1, [40], 0, 0, False),
+    (64, 3, 5, [333, 5, 63], 128, 0, False),
+    (64, 2, 16, [1000, 64], 128, 4, True),
+    (64, 1, 20, [500], 1, 0, False),
+    (128, 8, 4, [2000, 31, 0], 0, 0, False),
+    (128, 2, 12, [77, 300], 100, 33, True),
+    (128, 1, 128, [400], 0, 0, True),
+    (64, 1, 8, [200, 201], 64, 500, False),   # the first tokens cover everything
+    (64, 4, 8, [130, 17], 16, 1, False),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("splits", [None, 1, 3])
+@pytest.mark.parametrize("dim,kv_heads,group,before,window,first,with_sinks", SINGLE)
+def test_single_tokens(dtype, dim, kv_heads, group, before, window, first, with_sinks, splits):
+    new = [1] * len(before)
+    lengths, table, cache, query, sinks, offsets = make(
+        dim + group, dtype, dim, kv_heads, group, new, before, with_sinks=with_sinks)
+    out = call(query, cache, table, lengths, None, sinks, sliding_window=window or None,
+               first_tokens=first, splits=splits)
+    assert status() == 0
+    expected, bound = ref.attention(query, cache, table, lengths, offsets, sinks, window, first,
+                                    dim ** -0.5)
+    ref.assert_attention_close(out, expected, bound, dtype)
+    for b, m in enumerate(before):
+        if m is None:
+            assert (out[b] == 0).all()
+
+
+RUNS = [
+    # dim, kv_heads, group, new tokens, tokens before them, window, first, sinks
+    (64, 2, 8, [5, 1, 0, 3], [100, 0, 20, 1500], 0, 0, True),
+    (64, 1, 8, [200], [0], 0, 0, False),
+    (64, 2, 8, [130, 17, 64], [0, 300, 15], 0, 0, True),
+    (64, 1, 8, [300, 40], [50, 900], 128, 4, True),
+    (64, 1, 4, [150], [37], 20, 0, False),
+    (64, 2, 3, [90, 5], [10, 411], 0, 0, False),
+    (64, 1, 1, [257, 2], [1, 0], 0, 0, True),
+    (64, 1, 16, [33, 20], [0, 140], 50, 1, False),
+    (64, 1, 128, [7], [30], 0, 0, False),
+    (128, 2, 4, [140, 60], [3, 200], 0, 0, True),
+    (128, 1, 8, [100, 1], [0, 260], 64, 5, False),
+    (128, 1, 5, [70], [0], 0, 0, False),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("splits", [None, 1, 2])
+@pytest.mark.parametrize("dim,kv_heads,group,new,before,window,first,with_sinks", RUNS)
+def test_runs_of_tokens(dtype, dim, kv_heads, group, new, before, window, first, with_sinks,
+                        splits):
+    lengths, table, cache, query, sinks, offsets = make(
+        dim + group + 1, dtype, dim, kv_heads, group, new, before, with_sinks=with_sinks)
+    out = call(query, cache, table, lengths, offsets, sinks, sliding_window=window or None,
+               first_tokens=first, splits=splits)
+    assert status() == 0
+    expected, bound = ref.attention(query, cache, table, lengths, offsets, sinks, window, first,
+                                    dim ** -0.5)
+    ref.assert_attention_close(out, expected, bound, dtype)
+
+
+@pytest.mark.parametrize("runs", [False, True])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_blocks_of_unlike_magnitudes(dim, runs):
+    """Exponents of neighbouring blocks up to 2^40 apart, in keys and in values; queries of every
+    magnitude."""
+    new, before = ([60, 9], [200, 140]) if runs else ([1, 1], [259, 148])
+    lengths, table, cache, query, sinks, offsets = make(3, torch.bfloat16, dim, 2, 8, new, before,
+                                                        spread=20.0, with_sinks=True)
+    # keys of a common, small magnitude keep the softmax from collapsing onto one block
+    cache[1] = torch.full_like(cache[1], 120)
+    query = (query.float() * torch.exp2(torch.arange(query.shape[1]) % 7 - 3.0)[:, None]).to(
+        torch.bfloat16)
+    query[0, 0] *= 2.0 ** -90
+    query[0, 1] = 0
+    out = call(query, cache, table, lengths, offsets if runs else None, sinks)
+    assert status() == 0
+    expected, bound = ref.attention(query, cache, table, lengths, offsets, sinks, 0, 0,
+                                    dim ** -0.5)
+    ref.assert_attention_close(out, expected, bound, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_nan_tokens_reach_only_rows_that_see_them(dim):
+    """A row stored as NaN makes NaN of the queries that see it and leaves the others alone."""
+    new, before = [100], [30]
+    lengths, table, cache, query, sinks, offsets = make(4, torch.bfloat16, dim, 2, 8, new, before)
+    for token, at in ((70, 0), (90, 2)):  # a key row of head 0, a value row of head 1
+        page, slot = int(table[0, token // 16]), token % 16
+        cache[at][page, 0 if at == 0 else 1, slot] = 0x7f
+    out = call(query, cache, table, lengths, offsets, None)
+    assert status() == 0
+    expected, bound = ref.attention(query, cache, table, lengths, offsets, None, 0, 0, dim ** -0.5)
+    assert expected[40:, :8].isnan().all() and expected[60:, 8:].isnan().all()
+    assert not expected[:40].isnan().any() and not expected[:60, 8:].isnan().any()
+    ref.assert_attention_close(out, expected, bound, torch.bfloat16)
+    # single tokens, the NaN inside and outside a window
+    for window in (0, 10):
+        one = call(query[-1:], cache, table, lengths, None, None, sliding_window=window or None)
+        expected, bound = ref.attention(query[-1:], cache, table, lengths, [0, 1], None, window, 0,
+                                        dim ** -0.5)
+        assert expected.isnan().any() == (window == 0)
+        ref.assert_attention_close(one, expected, bound, torch.bfloat16)
+
+
+@pytest.mark.parametrize("splits", [1, 4])
+def test_rows_outside_every_sequence_stay(splits):
+    lengths, table, cache, query, sinks, _ = make(5, torch.float16, 64, 2, 8, [3, 0, 40, 9],
+                                                  [5, 7, 60, 100])
+    from nml_b200 import ops
+    offsets = [2, 3, 3, 41, 48]  # sequences of 1, 0, 38 and 7 rows
+    out = torch.full(query.shape, 5.0, dtype=torch.float16, device="cuda")
+    got = ops.paged_attention_q8(
+        query.cuda(), *[x.cuda() for x in cache], table.cuda(),
+        torch.tensor(lengths, dtype=torch.int32).cuda(),
+        query_offsets=torch.tensor(offsets, dtype=torch.int32).cuda(), splits=splits, out=out)
+    assert status() == 0 and got is out
+    expected, bound = ref.attention(query, cache, table, lengths, offsets, None, 0, 0, 0.125)
+    assert (out[:2] == 5).all() and (out[48:] == 5).all()
+    ref.assert_attention_close(out[2:48], expected[2:48], bound[2:48], torch.float16)
+
+
+@pytest.mark.parametrize("runs", [False, True])
+def test_more_rows_than_tokens(runs):
+    """Rows in front of a sequence's first token (a length below its row count) see nothing."""
+    new = [6, 4] if runs else [1, 1]
+    lengths, table, cache, query, sinks, offsets = make(6, torch.bfloat16, 64, 1, 8, new, [0, 30])
+    lengths[0] = 2 if runs else 0
+    out = call(query, cache, table, lengths, offsets if runs else None, None)
+    assert status() == 0
+    expected, bound = ref.attention(query, cache, table, lengths, offsets, None, 0, 0, 0.125)
+    assert (expected[: 4 if runs else 1] == 0).all()
+    ref.assert_attention_close(out, expected, bound, torch.bfloat16)
+
+
+@pytest.mark.parametrize("runs", [False, True])
+def test_bad_pages_are_reported_and_unseen(runs):
+    from nml_b200 import _abi
+    new, before = ([40], [60]) if runs else ([1], [99])
+    lengths, table, cache, query, sinks, offsets = make(7, torch.bfloat16, 64, 2, 8, new, before)
+    table[0, 2] = cache[0].shape[0]
+    table[0, 4] = -5
+    out = call(query, cache, table, lengths, offsets if runs else None, None)
+    assert status() == _abi.STATUS_INDEX_RANGE
+    assert torch.isfinite(out).all()
+    # a length past the table is cut to it
+    lengths, table, cache, query, sinks, offsets = make(8, torch.bfloat16, 64, 2, 8, new, before)
+    full = table.shape[1] * 16
+    out = call(query, cache, table, [full + 100], offsets if runs else None, None)
+    assert status() == _abi.STATUS_INDEX_RANGE
+    if not runs:
+        expected, bound = ref.attention(query, [torch.nan_to_num(x) for x in cache], table, [full],
+                                        offsets, None, 0, 0, 0.125)
+        assert torch.equal(out.isnan().cpu(), expected.isnan())
+
+
+def test_strided_queries_and_another_stream():
+    lengths, table, cache, query, sinks, offsets = make(9, torch.bfloat16, 64, 2, 8, [30, 50],
+                                                        [10, 500], with_sinks=True)
+    from nml_b200 import ops
+    wide = torch.zeros((80, 24, 64), dtype=torch.bfloat16, device="cuda")
+    wide[:, 4:20] = query.cuda()
+    dev = [x.cuda() for x in cache]
+    arguments = (*dev, table.cuda(), torch.tensor(lengths, dtype=torch.int32).cuda(),
+                 torch.tensor(offsets, dtype=torch.int32).cuda(), sinks.cuda())
+    plain = ops.paged_attention_q8(query.cuda(), *arguments)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        strided = ops.paged_attention_q8(wide[:, 4:20], *arguments)
+    torch.cuda.current_stream().wait_stream(side)
+    assert status() == 0
+    assert torch.equal(plain, strided)
+
+
+@pytest.mark.parametrize("runs", [False, True])
+def test_captured_graphs_share_no_scratch(runs):
+    """Two graphs captured on one stream, replayed at once on two streams, with splits."""
+    from nml_b200 import ops
+    sets = []
+    for seed in (10, 11):
+        new, before = ([20, 33], [900, 1500]) if runs else ([1, 1], [1900, 2400])
+        lengths, table, cache, query, sinks, offsets = make(seed, torch.bfloat16, 64, 2, 8, new,
+                                                            before)
+        dev = [x.cuda() for x in cache]
+        arguments = (query.cuda(), *dev, table.cuda(),
+                     torch.tensor(lengths, dtype=torch.int32).cuda(),
+                     torch.tensor(offsets, dtype=torch.int32).cuda() if runs else None)
+        eager = ops.paged_attention_q8(*arguments, splits=5)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.paged_attention_q8(*arguments, splits=5)
+        sets.append((graph, out, eager, arguments))
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for (graph, out, _, _), stream in zip(sets, streams):
+            with torch.cuda.stream(stream):
+                out.zero_()
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, out, eager, _ in sets:
+            assert torch.equal(out, eager)
+    assert status() == 0
+
+
+def test_prompts_and_tokens_in_a_row():
+    """A conversation: ragged prompts appended in two chunks and attended to, then single tokens,
+    each step against the 64-bit definition over the values read back from the cache."""
+    from nml_b200 import ops
+    gen = torch.Generator().manual_seed(12)
+    dtype, dim, kv_heads, group, batch = torch.bfloat16, 64, 2, 8, 3
+    total = [150, 40, 90]
+    table, pages = ref.random_table(gen, total)
+    cache = [x.cuda() for x in ref.stale(ref.random_cache(gen, pages, kv_heads, dim), table,
+                                         [0] * batch, gen)]
+    rotary = ops.rotary_table(150000.0 ** (-torch.arange(32, dtype=torch.float64) / 32), 200).cuda()
+    sinks = torch.randn(kv_heads * group, generator=gen)
+    lengths = [0] * batch
+    written = [torch.zeros((0, kv_heads, dim), dtype=torch.float64) for _ in range(batch)]
+    for step in ([100, 5, 33], [30, 20, 0], [1, 1, 1], [1, 1, 1]):
+        lengths = [m + n for m, n in zip(lengths, step)]
+        offsets = ref.offsets_of(step)
+        single = step == [1, 1, 1]
+        rows = torch.randn((sum(step), (group + 2) * kv_heads, dim), generator=gen).to(dtype)
+        fused = rows.cuda()
+        device_lengths = torch.tensor(lengths, dtype=torch.int32).cuda()
+        device_offsets = None if single else torch.tensor(offsets, dtype=torch.int32).cuda()
+        heads = group * kv_heads
+        query = ops.paged_append_q8(fused[:, heads:heads + kv_heads], fused[:, heads + kv_heads:],
+                                    *cache, table.cuda(), device_lengths, device_offsets,
+                                    query=fused[:, :heads], rotary=rotary)
+        out = ops.paged_attention_q8(query, *cache, table.cuda(), device_lengths, device_offsets,
+                                     sinks=sinks.cuda(), sliding_window=64, first_tokens=2)
+        assert status() == 0
+        held = [x.cpu() for x in cache]
+        expected, bound = ref.attention(query.cpu(), held, table, lengths, offsets, sinks, 64, 2,
+                                        dim ** -0.5)
+        ref.assert_attention_close(out, expected, bound, dtype)
+        for b in range(batch):
+            new = rows[offsets[b]:offsets[b + 1], heads + kv_heads:].double()
+            written[b] = torch.cat((written[b], new))
+            if lengths[b]:
+                # what the cache holds is what was written, to half a code step (2^-4) of each
+                # value or of the block's smallest code (two roundings where a block has grown)
+                value, _, exponent = ref.gather(held[2], held[3], table[b], lengths[b])
+                limit = written[b].abs() * 2.0 ** -4 * 1.07 + \
+                    2 * 2.0 ** -10 * torch.exp2(exponent)[..., None]
+                assert ((value - written[b]).abs() <= limit).all()
