@@ -21,27 +21,12 @@
 // tokens are interleaved byte-wise before they are widened.
 #include <type_traits>
 
-#include "cache_q8.cuh"
+#include "attention_q8.cuh"
 
 namespace nml_sm100 {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr float kLog2e = 1.4426950408889634f;
-
-struct AttentionParams {
-  CacheQ8 cache;
-  const void* query;
-  const int32_t* offsets;  // [batch + 1] or null
-  const float* sinks;
-  float* partial;          // [rows, query_heads, splits, D + 2]: out, maximum, sum
-  void* output;
-  int64_t query_token_stride, query_head_stride;
-  int tokens, query_heads, group, head_tiles, splits, window, first;
-  float scale_log2;
-  int* status;
-};
-
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -56,24 +41,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
-}
-
-// Which logical pages a row sees: [0, front) and [back, end), and its token limits.
-struct Visible {
-  int length;  // tokens in front of (and with) the row's own
-  int start;   // first token of the window
-  int front, back, pages;
-};
-
-__device__ __forceinline__ Visible visible_pages(int length, int window, int first) {
-  Visible v;
-  v.length = max(length, 0);
-  v.start = window > 0 ? max(0, v.length - window) : 0;
-  const int end = (v.length + kCachePage - 1) / kCachePage;
-  v.back = v.start / kCachePage;
-  v.front = v.start > 0 ? min((first + kCachePage - 1) / kCachePage, v.back) : 0;
-  v.pages = v.front + end - v.back;
-  return v;
 }
 
 // NT: tiles of 8 query heads of one kv head that share the loaded codes.
@@ -96,7 +63,7 @@ row_kernel(const AttentionParams p) {
   if (sequence < 0) return;  // a row of no sequence is left as it was
   int length = sequence_length(p.cache, sequence, p.status);
   if (p.offsets != nullptr) length += row + 1 - p.offsets[sequence + 1];
-  const Visible v = visible_pages(length, p.window, p.first);
+  const Visible v = visible_pages(length, p.window > 0 ? length - p.window : 0, p.first);
   const int per_split = (v.pages + p.splits - 1) / p.splits;
   const int page_begin = split * per_split;
   const int page_end = min(v.pages, page_begin + per_split);
@@ -141,9 +108,7 @@ row_kernel(const AttentionParams p) {
       }
       largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
       largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-      // power of two that puts the row's largest into [2^14, 2^15); none for zeros, NaN, infinity
-      int shift = 14 - (static_cast<int>(largest >> 23) - 127);
-      shift = largest == 0 || largest >= 0x7f800000u ? 0 : min(shift, 100);
+      const int shift = query_shift(largest);
       const float up = exp2_int(shift);
       inverse = exp2_int(-shift);
 #pragma unroll
@@ -318,7 +283,7 @@ row_kernel(const AttentionParams p) {
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
         m = fmaxf(m, running_max[n][j]);
         // nothing seen yet: leave the (empty) state as it is
-        const float rescale = m == -INFINITY ? 1.0f : exp2f(running_max[n][j] - m);
+        const float rescale = m == -INFINITY ? 1.0f : exp2_fast(running_max[n][j] - m);
         base[n][j] = m == -INFINITY ? 0.0f : m;
         running_max[n][j] = m;
         running_sum[n][j] *= rescale;
@@ -331,14 +296,14 @@ row_kernel(const AttentionParams p) {
     }
 #pragma unroll
     for (int i = 0; i < CP; ++i) {
-      const float unscale = exp2f(-value_exponent[i]);
+      const float unscale = exp2_fast(-value_exponent[i]);
       uint32_t weights[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const float w0 = exp2f(s[n][i][0] + (value_exponent[i] - base[n][0]));
-        const float w1 = exp2f(s[n][i][1] + (value_exponent[i] - base[n][1]));
-        const float w2 = exp2f(s[n][i][2] + (value_exponent[i] - base[n][0]));
-        const float w3 = exp2f(s[n][i][3] + (value_exponent[i] - base[n][1]));
+        const float w0 = exp2_fast(s[n][i][0] + (value_exponent[i] - base[n][0]));
+        const float w1 = exp2_fast(s[n][i][1] + (value_exponent[i] - base[n][1]));
+        const float w2 = exp2_fast(s[n][i][2] + (value_exponent[i] - base[n][0]));
+        const float w3 = exp2_fast(s[n][i][3] + (value_exponent[i] - base[n][1]));
         running_sum[n][0] = fmaf(w0 + w2, unscale, running_sum[n][0]);
         running_sum[n][1] = fmaf(w1 + w3, unscale, running_sum[n][1]);
         weights[n][0] = transpose8x8(Elem<__half>::pack2(w0, w1));
@@ -468,10 +433,14 @@ join_kernel(const AttentionParams p) {
 }
 
 template <typename T, int D>
-void launch_rows(const AttentionParams& p, cudaStream_t stream) {
+int32_t launch_attention(const AttentionParams& p, bool tiles, cudaStream_t stream, char* message,
+                         size_t capacity) {
   const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(p.tokens) * p.splits),
                   static_cast<unsigned>(p.cache.kv_heads * p.head_tiles));
-  if (p.group <= 8) {
+  if (tiles) {
+    const int32_t code = launch_tiles<T, D>(p, stream, message, capacity);
+    if (code != NML_SM100_OK) return code;
+  } else if (p.group <= 8) {
     row_kernel<T, D, 1, 256 / D><<<grid, kWarps * 32, 0, stream>>>(p);
   } else {
     row_kernel<T, D, 2, 128 / D><<<grid, kWarps * 32, 0, stream>>>(p);
@@ -480,6 +449,7 @@ void launch_rows(const AttentionParams& p, cudaStream_t stream) {
     const int64_t heads = static_cast<int64_t>(p.tokens) * p.query_heads;
     join_kernel<T, D><<<static_cast<unsigned>((heads + 3) / 4), 128, 0, stream>>>(p);
   }
+  return launch_result(message, capacity);
 }
 
 // Pages that a row can see at most.
@@ -490,11 +460,19 @@ int64_t most_pages(const NmlSm100PagedAttentionQ8& r) {
   return pages < r.cache.table_width ? pages : r.cache.table_width;
 }
 
+// Runs of tokens go to the tile kernel, single tokens to the row kernel.
+bool use_tiles(const NmlSm100PagedAttentionQ8& r) {
+  return r.query_offsets != nullptr && r.tokens > r.cache.batch;
+}
+
 // Splits of the visible pages: until there are two CTAs for every SM, at least eight pages each.
 int64_t choose_splits(const NmlSm100PagedAttentionQ8& r) {
   if (r.splits > 0) return r.splits;
   constexpr int64_t kWanted = 2 * 148;
-  const int64_t pairs = r.tokens * r.cache.kv_heads;
+  const int64_t pairs =
+      r.cache.kv_heads * (use_tiles(r) ? query_tiles(r.tokens, r.cache.batch,
+                                                     r.query_heads / r.cache.kv_heads)
+                                       : r.tokens);
   int64_t splits = (kWanted + pairs - 1) / pairs;
   const int64_t most = most_pages(r) / 8;
   if (splits > most) splits = most;
@@ -556,7 +534,9 @@ extern "C" int32_t nml_sm100_paged_attention_q8(const NmlSm100PagedAttentionQ8* 
                 error_message, error_message_capacity);
   }
   const int64_t splits = choose_splits(r);
-  if (r.tokens * splits > std::numeric_limits<int32_t>::max()) {
+  if (r.tokens * splits > std::numeric_limits<int32_t>::max() ||
+      (r.tokens + r.cache.batch) * splits * r.cache.kv_heads >
+          std::numeric_limits<int32_t>::max()) {
     return fail(NML_SM100_INVALID_ARGUMENT, "invalid 8-bit paged attention request: too many rows",
                 error_message, error_message_capacity);
   }
@@ -587,10 +567,15 @@ extern "C" int32_t nml_sm100_paged_attention_q8(const NmlSm100PagedAttentionQ8* 
   p.status = device->status_word;
   cudaStream_t stream = static_cast<cudaStream_t>(r.stream);
   const bool half = r.dtype == NML_SM100_F16;
+  const bool tiles = use_tiles(r);
   if (r.cache.head_dim == 64) {
-    half ? launch_rows<__half, 64>(p, stream) : launch_rows<__nv_bfloat16, 64>(p, stream);
-  } else {
-    half ? launch_rows<__half, 128>(p, stream) : launch_rows<__nv_bfloat16, 128>(p, stream);
+    return half ? launch_attention<__half, 64>(p, tiles, stream, error_message,
+                                               error_message_capacity)
+                : launch_attention<__nv_bfloat16, 64>(p, tiles, stream, error_message,
+                                                      error_message_capacity);
   }
-  return launch_result(error_message, error_message_capacity);
+  return half ? launch_attention<__half, 128>(p, tiles, stream, error_message,
+                                              error_message_capacity)
+              : launch_attention<__nv_bfloat16, 128>(p, tiles, stream, error_message,
+                                                     error_message_capacity);
 }

@@ -1,0 +1,70 @@
+// What the two kernels of attention over the 8-bit paged cache share: one row at a time
+// (attention_q8.cu) and tiles of rows on the tensor cores (attention_q8_tile.cu).
+#pragma once
+
+#include "cache_q8.cuh"
+
+namespace nml_sm100 {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct AttentionParams {
+  CacheQ8 cache;
+  const void* query;
+  const int32_t* offsets;  // [batch + 1] or null
+  const float* sinks;
+  float* partial;          // [rows, query_heads, splits, D + 2]: out, maximum, sum
+  void* output;
+  int64_t query_token_stride, query_head_stride;
+  int tokens, query_heads, group, head_tiles, splits, window, first;
+  float scale_log2;
+  int* status;
+};
+
+// 2^x to 2 units in the last place (CUDA's documented bound of ex2.approx); results below 2^-126
+// are zero.  exp2f() itself would spend two more instructions on those.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Power of two that puts the largest magnitude of a BF16 row (given as f32 bits) into
+// [2^14, 2^15), so that the row's narrowing to F16 is exact down to 2^-29 of it; none for rows of
+// zeros or with an infinity or a NaN.
+__device__ __forceinline__ int query_shift(uint32_t largest_bits) {
+  const int shift = 14 - (static_cast<int>(largest_bits >> 23) - 127);
+  return largest_bits == 0 || largest_bits >= 0x7f800000u ? 0 : min(shift, 100);
+}
+
+// Which logical pages queries see: [0, front) and [back, end), of `pages` entries in this order.
+struct Visible {
+  int length;  // tokens in front of (and with) the last query's own
+  int start;   // first token of the first query's window
+  int front, back, pages;
+};
+
+__device__ __forceinline__ Visible visible_pages(int length, int start, int first) {
+  Visible v;
+  v.length = max(length, 0);
+  v.start = max(start, 0);
+  const int end = (v.length + kCachePage - 1) / kCachePage;
+  v.back = min(v.start / kCachePage, end);
+  v.front = v.start > 0 ? min((first + kCachePage - 1) / kCachePage, v.back) : 0;
+  v.pages = v.front + end - v.back;
+  return v;
+}
+
+// Rows of a query tile of the tile kernel and the number of its work items (an upper bound that
+// needs no device data).
+constexpr int kTileRows = 128;
+inline int64_t query_tiles(int64_t tokens, int64_t batch, int64_t group) {
+  const int64_t per_tile = kTileRows / group;
+  return tokens / per_tile + (batch < tokens ? batch : tokens);
+}
+
+template <typename T, int D>
+int32_t launch_tiles(const AttentionParams& p, cudaStream_t stream, char* message,
+                     size_t capacity);
+
+}  // namespace nml_sm100
