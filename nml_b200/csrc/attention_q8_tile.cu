@@ -8,10 +8,12 @@
 //   warps 0-3  softmax, one thread for each row: q into tensor memory (F16, a power of two for the
 //              row), then for every step the scores out of tensor memory, maximum, weights back
 //              into tensor memory over the scores; rescales the accumulator when needed
-//   warp 4     issues the products: S = Q K^T (A: q in tensor memory, B: keys, K-major) and
+//   warps 4-7  widen the codes: 16-byte loads, E4M3 to F16 (exact, the block scales stay out),
+//              128-byte swizzled stores; the next step's loads are in flight meanwhile, page
+//              table entries and scales are fetched for 32 pages at a time, 32 pages ahead
+//   warp 8     issues the products: S = Q K^T (A: q in tensor memory, B: keys, K-major) and
 //              O += W V (A: weights in tensor memory, B: values, MN-major: tokens are rows)
-//   warps 5-7  widen the codes: 16-byte loads, E4M3 to F16 (exact, the block scales stay out),
-//              128-byte swizzled stores; the next step's loads are in flight meanwhile
+// Registers move from the last two warpgroups to the softmax, which holds a row's 64 scores.
 //
 // The running maximum M only stabilises: weights reach up to 2^8 before it is raised (F16 holds
 // them, sums are f32), so the accumulator in tensor memory is rescaled a few times for a row and
@@ -31,9 +33,11 @@ namespace {
 constexpr int kStepTokens = 64;
 constexpr int kStepPages = kStepTokens / kCachePage;
 constexpr int kSoftmaxThreads = 128;
-constexpr int kMmaWarp = 4;
-constexpr int kWidenWarps = 3;
-constexpr int kThreads = 256;
+constexpr int kWidenThreads = 128;
+constexpr int kWidenWarp = 4;
+constexpr int kMmaWarp = 8;
+constexpr int kThreads = 384;  // the last three warps only give their registers
+constexpr int kLaunchRegisters = 80;  // of a thread: two CTAs fill an SM
 constexpr float kSlack = 8.0f;  // log2 of the largest weight before the maximum is raised
 constexpr int kTmemColumns = 256;
 
@@ -55,6 +59,12 @@ struct Shape {
   static constexpr int kBuffers = D == 64 ? 2 : 1;  // score buffers in tensor memory
   static constexpr int kOut = 0, kQuery = D, kScores = D + D / 2;
   static constexpr int kSharedBytes = kStages * 2 * kTileBytes + 1024;
+  // The three warpgroups' shares of the CTA's registers at launch.
+  static constexpr int kSoftmaxRegisters = D == 64 ? 144 : 136;
+  static constexpr int kWidenRegisters = D == 64 ? 72 : 80;
+  static constexpr int kMmaRegisters = 24;
+  static_assert(kSoftmaxRegisters + kWidenRegisters + kMmaRegisters == 3 * kLaunchRegisters,
+                "a share that the launch does not cover would be waited for without end");
   static_assert(kScores + kBuffers * kStepTokens <= kTmemColumns, "tensor memory");
 };
 
@@ -70,6 +80,35 @@ struct Control {
   alignas(16) uint32_t any_nan[Shape<D>::kStages][4];  // read 16 bytes at a time
   uint8_t row_nan[Shape<D>::kStages][kStepTokens];
 };
+
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// Two f32 at a time.
+__device__ __forceinline__ uint64_t pack_f32x2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack_f32x2(uint64_t x, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x));
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -118,7 +157,7 @@ tile_kernel(const AttentionParams p) {
   }
   if (threadIdx.x == kMmaWarp * 32) {
     for (int i = 0; i < S::kStages; ++i) {
-      mbar_init(&control.tiles_full[i], kWidenWarps * 32);
+      mbar_init(&control.tiles_full[i], kWidenThreads);
       mbar_init(&control.tiles_free[i], 1);
     }
     for (int i = 0; i < S::kBuffers; ++i) mbar_init(&control.scores_full[i], 1);
@@ -160,8 +199,9 @@ tile_kernel(const AttentionParams p) {
     __syncwarp();
   };
 
-  if (warp < kMmaWarp) {
+  if (warp < kWidenWarp) {
     // ------------------------------------------------------------------ softmax
+    more_registers<S::kSoftmaxRegisters>();
     const int row = threadIdx.x;
     const int token = row / p.group;
     const int head = kv_head * p.group + row - token * p.group;
@@ -228,20 +268,18 @@ tile_kernel(const AttentionParams p) {
       tcgen05_fence_after_sync();
       // long complete; orders the reads of the stage's page data behind their writes
       wait(&control.tiles_full[stage], j / S::kStages, kSiteTiles);
+      uint32_t scores_lo[32], scores_hi[32];
+      tmem_load_32x32(columns, scores_lo);
+      tmem_load_32x32(columns + 32, scores_hi);
+      tmem_load_wait();
       float s[kStepTokens];
-      {
-        uint32_t x[32];
-        tmem_load_32x32(columns, x);
-        tmem_load_wait();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) s[i] = __uint_as_float(x[i]);
-        tmem_load_32x32(columns + 32, x);
-        tmem_load_wait();
-#pragma unroll
-        for (int i = 0; i < 32; ++i) s[32 + i] = __uint_as_float(x[i]);
+      for (int i = 0; i < 32; ++i) {
+        s[i] = __uint_as_float(scores_lo[i]);
+        s[32 + i] = __uint_as_float(scores_hi[i]);
       }
       const uint4 nan_words = *reinterpret_cast<const uint4*>(control.any_nan[stage]);
-      bool whole = (nan_words.x | nan_words.y | nan_words.z) == 0;
+      bool whole = (nan_words.x | nan_words.y | nan_words.z | nan_words.w) == 0;
 #pragma unroll
       for (int q = 0; q < kStepPages; ++q) {
         const int t = control.pages[stage][q].token;
@@ -299,16 +337,25 @@ tile_kernel(const AttentionParams p) {
 #pragma unroll
       for (int q = 0; q < kStepPages; ++q) {
         const float offset = control.pages[stage][q].value_exponent - base;
+        const uint64_t factor2 = pack_f32x2(page_factor[q], page_factor[q]);
+        const uint64_t offset2 = pack_f32x2(offset, offset);
         uint32_t packed[8];
-        float sum = 0.0f;
+        uint64_t sum2 = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float a = exp2_fast(fmaf(s[q * kCachePage + 2 * i], page_factor[q], offset));
-          const float b = exp2_fast(fmaf(s[q * kCachePage + 2 * i + 1], page_factor[q], offset));
-          sum += a + b;
+          float a, b;
+          unpack_f32x2(fma_f32x2(pack_f32x2(s[q * kCachePage + 2 * i],
+                                            s[q * kCachePage + 2 * i + 1]),
+                                 factor2, offset2),
+                       a, b);
+          a = exp2_fast(a);
+          b = exp2_fast(b);
+          sum2 = add_f32x2(sum2, pack_f32x2(a, b));
           packed[i] = Elem<__half>::pack2(a, b);
         }
-        running_sum = fmaf(sum, control.pages[stage][q].unscale, running_sum);
+        float sum_even, sum_odd;
+        unpack_f32x2(sum2, sum_even, sum_odd);
+        running_sum = fmaf(sum_even + sum_odd, control.pages[stage][q].unscale, running_sum);
         tmem_store_32x8(columns + 8 * q, packed);
       }
       tmem_store_wait();
@@ -362,147 +409,182 @@ tile_kernel(const AttentionParams p) {
     if (live && p.splits > 1) {
       *reinterpret_cast<float2*>(partial + D) = make_float2(running_max, running_sum);
     }
-  } else if (warp == kMmaWarp) {
+  } else if (warp >= kMmaWarp) {
     // ------------------------------------------------------------------ matrix products
-    constexpr uint64_t desc_hi = static_cast<uint64_t>(kUmmaDescHiSw128) << 32;
-    constexpr uint32_t score_idesc = umma_idesc_f16(kUmmaF16, kUmmaF16, kTileRows, kStepTokens);
-    constexpr uint32_t product_idesc =
-        umma_idesc_f16(kUmmaF16, kUmmaF16, kTileRows, D) | (1u << 16);  // B is MN-major
-    auto scores = [&](int j) {
-      const int stage = j % S::kStages, buffer = j % S::kBuffers;
-      wait(&control.tiles_full[stage], j / S::kStages, kSiteTiles);
-      tcgen05_fence_after_sync();
-      const uint32_t keys = smem_u32(shared + stage * 2 * S::kTileBytes);
+    fewer_registers<S::kMmaRegisters>();
+    if (warp == kMmaWarp) {
+      constexpr uint64_t desc_hi = static_cast<uint64_t>(kUmmaDescHiSw128) << 32;
+      constexpr uint32_t score_idesc = umma_idesc_f16(kUmmaF16, kUmmaF16, kTileRows, kStepTokens);
+      constexpr uint32_t product_idesc =
+          umma_idesc_f16(kUmmaF16, kUmmaF16, kTileRows, D) | (1u << 16);  // B is MN-major
+      auto scores = [&](int j) {
+        const int stage = j % S::kStages, buffer = j % S::kBuffers;
+        wait(&control.tiles_full[stage], j / S::kStages, kSiteTiles);
+        tcgen05_fence_after_sync();
+        const uint32_t keys = smem_u32(shared + stage * 2 * S::kTileBytes);
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        // 64-element halves of the head are tiles of their own, 16 elements are 32 bytes of a row
-        const uint32_t address = keys + (k / 4) * (kStepTokens * 128) + (k % 4) * 32;
-        umma_f16_tmem_a_elect(tmem + S::kScores + buffer * kStepTokens, tmem + S::kQuery + 8 * k,
-                              desc_hi | umma_desc_lo(address), score_idesc, k > 0 ? 1u : 0u);
+        for (int k = 0; k < D / 16; ++k) {
+          // 64-element halves of the head are tiles of their own, 16 elements are 32 bytes of a row
+          const uint32_t address = keys + (k / 4) * (kStepTokens * 128) + (k % 4) * 32;
+          umma_f16_tmem_a_elect(tmem + S::kScores + buffer * kStepTokens, tmem + S::kQuery + 8 * k,
+                                desc_hi | umma_desc_lo(address), score_idesc, k > 0 ? 1u : 0u);
+        }
+        umma_commit_elect(&control.scores_full[buffer]);
+      };
+      if (steps > 0) {
+        wait(&control.query_full, 0, kSiteWeights);
+        tcgen05_fence_after_sync();
+        for (int j = 0; j < min(steps, S::kBuffers); ++j) scores(j);
       }
-      umma_commit_elect(&control.scores_full[buffer]);
-    };
-    if (steps > 0) {
-      wait(&control.query_full, 0, kSiteWeights);
-      tcgen05_fence_after_sync();
-      for (int j = 0; j < min(steps, S::kBuffers); ++j) scores(j);
-    }
-    for (int j = 0; j < steps; ++j) {
-      const int stage = j % S::kStages, buffer = j % S::kBuffers;
-      wait(&control.weights_full, j, kSiteWeights);
-      tcgen05_fence_after_sync();
-      const uint32_t values = smem_u32(shared + stage * 2 * S::kTileBytes + S::kTileBytes);
+      for (int j = 0; j < steps; ++j) {
+        const int stage = j % S::kStages, buffer = j % S::kBuffers;
+        wait(&control.weights_full, j, kSiteWeights);
+        tcgen05_fence_after_sync();
+        const uint32_t values = smem_u32(shared + stage * 2 * S::kTileBytes + S::kTileBytes);
 #pragma unroll
-      for (int k = 0; k < kStepTokens / 16; ++k) {
-        // 16 tokens are 2 KB of 128-byte rows; the leading offset is the next 64 dimensions' tile
-        const uint32_t address = values + k * 2048;
-        const uint32_t low = ((address & 0x3ffffu) >> 4) | ((kStepTokens * 128 >> 4) << 16);
-        umma_f16_tmem_a_elect(tmem + S::kOut, tmem + S::kScores + buffer * kStepTokens + 8 * k,
-                              desc_hi | low, product_idesc, j > 0 || k > 0 ? 1u : 0u);
+        for (int k = 0; k < kStepTokens / 16; ++k) {
+          // 16 tokens are 2 KB of 128-byte rows; the leading offset is the next 64 dimensions' tile
+          const uint32_t address = values + k * 2048;
+          const uint32_t low = ((address & 0x3ffffu) >> 4) | ((kStepTokens * 128 >> 4) << 16);
+          umma_f16_tmem_a_elect(tmem + S::kOut, tmem + S::kScores + buffer * kStepTokens + 8 * k,
+                                desc_hi | low, product_idesc, j > 0 || k > 0 ? 1u : 0u);
+        }
+        umma_commit_elect(&control.tiles_free[stage]);
+        umma_commit_elect(&control.product_done);
+        if (j + S::kBuffers < steps) {
+          // the scores go over the weights that this product reads
+          wait(&control.product_done, j, kSiteProduct);
+          scores(j + S::kBuffers);
+        }
       }
-      umma_commit_elect(&control.tiles_free[stage]);
-      umma_commit_elect(&control.product_done);
-      if (j + S::kBuffers < steps) {
-        // the scores go over the weights that this product reads
-        wait(&control.product_done, j, kSiteProduct);
-        scores(j + S::kBuffers);
+      umma_commit_elect(&control.drained);
+      if (!mbar_wait(&control.drained, 0)) {
+        *abort_flag = 1;
+        atomicOr(p.status, NML_SM100_STATUS_BARRIER_TIMEOUT | (0x100 << kSiteProduct));
       }
-    }
-    umma_commit_elect(&control.drained);
-    if (!mbar_wait(&control.drained, 0)) {
-      *abort_flag = 1;
-      atomicOr(p.status, NML_SM100_STATUS_BARRIER_TIMEOUT | (0x100 << kSiteProduct));
     }
   } else {
     // ------------------------------------------------------------------ codes to F16 tiles
-    constexpr int kWidenThreads = kWidenWarps * 32;
-    constexpr int kRowPieces = D / 16;                  // pieces of 16 codes of a token's row
-    constexpr int kHalf = kStepTokens * kRowPieces;     // pieces of the keys (then of the values)
-    constexpr int kRounds = (2 * kHalf + kWidenThreads - 1) / kWidenThreads;
-    const int thread = threadIdx.x - (kMmaWarp + 1) * 32;
-    const int widen_warp = warp - kMmaWarp - 1;
+    fewer_registers<S::kWidenRegisters>();
+    constexpr int kParts = D / 16;                          // pieces of 16 codes of a token's row
+    constexpr int kTokens = kWidenThreads / kParts;         // tokens of one load of the group
+    constexpr int kRounds = kStepTokens / kTokens;          // loads for the keys of a step
+    constexpr int kGroup = 32;                              // pages looked up at once
+    const int thread = threadIdx.x - kWidenWarp * 32;
+    const int part = thread % kParts, first_token = thread / kParts;
+    // page of round r's token: r * (kTokens / 16) + lane_page
+    const int lane_page = first_token / kCachePage;
+    const uint32_t head_bytes = kCachePage * D;
+    const int64_t page_bytes = static_cast<int64_t>(p.cache.kv_heads) * head_bytes;
+    const int64_t thread_bytes = static_cast<int64_t>(kv_head) * head_bytes +
+                                 (first_token % kCachePage) * D + part * 16;
+    const uint8_t* const key_codes = p.cache.codes[0] + thread_bytes;
+    const uint8_t* const value_codes = p.cache.codes[1] + thread_bytes;
+    uint8_t* const own_tile = shared + (part / 4) * (kStepTokens * 128) + first_token * 128;
+    // 16-byte chunks 2 part and 2 part + 1 of a 128-byte row, swizzled by the token
+    const int chunk_lo = ((2 * (part % 4)) ^ (first_token & 7)) * 16;
+    const int chunk_hi = ((2 * (part % 4) + 1) ^ (first_token & 7)) * 16;
 
-    // lane q < 4 holds what page q of a step is: its block (-1: nothing there) and scale bytes
-    int64_t block = -1;
-    PageInfo info;
-    auto look_up = [&](int j) {
-      block = -1;
-      info = PageInfo{0.0f, -INFINITY, 0.0f, -kStepTokens};  // a page of nobody: weights of zero
-      const int i = (step_begin + j) * kStepPages + lane;
-      if (lane < kStepPages && j < steps && i < v.pages) {
-        const int logical = i < v.front ? i : i - v.front + v.back;
-        const int page = physical_page(p.cache, sequence, logical, p.status);
+    // lane i holds page (-1: nothing there) and scale bytes of entry i of a group of 32
+    auto look_up = [&](int group, int& page, uint32_t& bytes) {
+      page = -1;
+      bytes = 0;
+      const int i = group * kGroup + lane;
+      if (i >= step_begin * kStepPages && i < min(v.pages, (step_begin + steps) * kStepPages)) {
+        page = physical_page(p.cache, sequence, i < v.front ? i : i - v.front + v.back, p.status);
         if (page >= 0) {
-          block = static_cast<int64_t>(page) * p.cache.kv_heads + kv_head;
-          const int e = scale_exponent(p.cache.scales[1][block]);
-          info = PageInfo{exp2_int(scale_exponent(p.cache.scales[0][block])),
-                          static_cast<float>(e), exp2_int(-e), logical * kCachePage};
+          const int64_t block = static_cast<int64_t>(page) * p.cache.kv_heads + kv_head;
+          bytes = p.cache.scales[0][block] | static_cast<uint32_t>(p.cache.scales[1][block]) << 8;
         }
       }
     };
-    uint4 codes[kRounds];
-    auto load = [&](uint4 (&to)[kRounds]) {
+    constexpr int kSteps = kGroup / kStepPages;  // steps of a group of pages
+    int group = step_begin / kSteps;
+    int page, next_page;          // of this group and of the one behind it
+    uint32_t bytes, next_bytes;
+    look_up(group, page, bytes);
+    look_up(group + 1, next_page, next_bytes);
+
+    auto load = [&](int j, uint4 (&keys)[kRounds], uint4 (&values)[kRounds]) {
+      const int step = step_begin + j;
+      const int held = step / kSteps == group ? page : next_page;
+      const int at = step % kSteps * kStepPages + lane_page;
 #pragma unroll
       for (int r = 0; r < kRounds; ++r) {
-        const int piece = r * kWidenThreads + thread;
-        const int within = piece % kHalf;
-        const int token = within / kRowPieces;
-        const int64_t b = __shfl_sync(0xffffffffu, block, token / kCachePage);
-        to[r] = make_uint4(0, 0, 0, 0);
-        if (piece < 2 * kHalf && b >= 0) {
-          const uint8_t* base = piece < kHalf ? p.cache.codes[0] : p.cache.codes[1];
-          to[r] = *reinterpret_cast<const uint4*>(base + b * (kCachePage * D) +
-                                                  (token % kCachePage) * D +
-                                                  (within % kRowPieces) * 16);
+        const int q = __shfl_sync(0xffffffffu, held, at + r * (kTokens / kCachePage));
+        keys[r] = values[r] = make_uint4(0, 0, 0, 0);
+        if (q >= 0) {
+          keys[r] = *reinterpret_cast<const uint4*>(key_codes + q * page_bytes);
+          values[r] = *reinterpret_cast<const uint4*>(value_codes + q * page_bytes);
         }
       }
     };
-    look_up(0);
-    load(codes);
-    for (int j = 0; j < steps; ++j) {
+    auto widen = [](uint8_t* row, int lo, int hi, const uint4& x) {
+      *reinterpret_cast<uint4*>(row + lo) =
+          make_uint4(e4m3x2_to_f16x2(x.x & 0xffffu), e4m3x2_to_f16x2(x.x >> 16),
+                     e4m3x2_to_f16x2(x.y & 0xffffu), e4m3x2_to_f16x2(x.y >> 16));
+      *reinterpret_cast<uint4*>(row + hi) =
+          make_uint4(e4m3x2_to_f16x2(x.z & 0xffffu), e4m3x2_to_f16x2(x.z >> 16),
+                     e4m3x2_to_f16x2(x.w & 0xffffu), e4m3x2_to_f16x2(x.w >> 16));
+    };
+    auto put = [&](int j, const uint4 (&keys)[kRounds], const uint4 (&values)[kRounds]) {
       const int stage = j % S::kStages;
-      const PageInfo current = info;
-      look_up(j + 1);
-      uint4 next[kRounds];
-      load(next);
+      const int step = step_begin + j;
+      const int entry = step * kStepPages;
       if (j >= S::kStages) wait(&control.tiles_free[stage], j / S::kStages - 1, kSiteFree);
-      uint8_t* const tiles = shared + stage * 2 * S::kTileBytes;
+      uint8_t* const tile = own_tile + stage * 2 * S::kTileBytes;
       bool any_nan = false;
 #pragma unroll
       for (int r = 0; r < kRounds; ++r) {
-        const int piece = r * kWidenThreads + thread;
-        const int within = piece % kHalf;
-        const int token = within / kRowPieces, part = within % kRowPieces;
-        uint4 x = codes[r];
-        const int page_token =
-            __shfl_sync(0xffffffffu, current.token, token / kCachePage) + token % kCachePage;
-        const uint32_t first_code = __shfl_sync(0xffffffffu, x.x, lane & ~(kRowPieces - 1));
-        if (piece < 2 * kHalf) {
-          if (piece >= kHalf) {
-            // values that no row sees, or that are NaN, must not meet the product
-            const bool nan = (first_code & 0x7fu) == 0x7fu && page_token < v.length;
-            if (nan || page_token >= v.length) x = make_uint4(0, 0, 0, 0);
-            if (part == 0) control.row_nan[stage][token] = nan ? 1 : 0;
-            any_nan = any_nan || nan;
-          }
-          uint8_t* const tile = tiles + (piece < kHalf ? 0 : S::kTileBytes) +
-                                (part / 4) * (kStepTokens * 128) + token * 128;
-          const int chunk = 2 * (part % 4);
-          *reinterpret_cast<uint4*>(tile + ((chunk ^ (token & 7)) * 16)) =
-              make_uint4(e4m3x2_to_f16x2(x.x & 0xffffu), e4m3x2_to_f16x2(x.x >> 16),
-                         e4m3x2_to_f16x2(x.y & 0xffffu), e4m3x2_to_f16x2(x.y >> 16));
-          *reinterpret_cast<uint4*>(tile + (((chunk + 1) ^ (token & 7)) * 16)) =
-              make_uint4(e4m3x2_to_f16x2(x.z & 0xffffu), e4m3x2_to_f16x2(x.z >> 16),
-                         e4m3x2_to_f16x2(x.w & 0xffffu), e4m3x2_to_f16x2(x.w >> 16));
-        }
+        const int token = r * kTokens + first_token;
+        const int i = entry + r * (kTokens / kCachePage) + lane_page;
+        const int position = (i < v.front ? i : i - v.front + v.back) * kCachePage +
+                             first_token % kCachePage;
+        // values that no row sees, or that are NaN (the whole row then), must not meet the product
+        const bool unseen = position >= v.length;
+        const bool nan = (values[r].x & 0x7fu) == 0x7fu && !unseen;
+        any_nan = any_nan || nan;
+        if (part == 0) control.row_nan[stage][token] = nan ? 1 : 0;
+        widen(tile + r * kTokens * 128, chunk_lo, chunk_hi, keys[r]);
+        widen(tile + S::kTileBytes + r * kTokens * 128, chunk_lo, chunk_hi,
+              nan || unseen ? make_uint4(0, 0, 0, 0) : values[r]);
       }
       any_nan = __any_sync(0xffffffffu, any_nan);
-      if (lane == 0) control.any_nan[stage][widen_warp] = any_nan ? 1u : 0u;
-      if (widen_warp == 0 && lane < kStepPages) control.pages[stage][lane] = current;
+      if (lane == 0) control.any_nan[stage][warp - kWidenWarp] = any_nan ? 1u : 0u;
+      if (warp == kWidenWarp) {
+        const int at = step % kSteps * kStepPages + (lane & (kStepPages - 1));
+        const int held = __shfl_sync(0xffffffffu, page, at);
+        const uint32_t scales = __shfl_sync(0xffffffffu, bytes, at);
+        if (lane < kStepPages) {
+          // a page of nobody gives weights of zero and asks for no masks
+          PageInfo info{0.0f, -INFINITY, 0.0f, -kStepTokens};
+          if (held >= 0) {
+            const int i = entry + lane;
+            const int e = scale_exponent(scales >> 8);
+            info = PageInfo{exp2_int(scale_exponent(scales & 0xffu)), static_cast<float>(e),
+                            exp2_int(-e), (i < v.front ? i : i - v.front + v.back) * kCachePage};
+          }
+          control.pages[stage][lane] = info;
+        }
+      }
       fence_proxy_async_smem();
       mbar_arrive(&control.tiles_full[stage]);
-#pragma unroll
-      for (int r = 0; r < kRounds; ++r) codes[r] = next[r];
+      if ((step + 1) % kSteps == 0) {  // on to the next group of pages
+        ++group;
+        page = next_page;
+        bytes = next_bytes;
+        look_up(group + 1, next_page, next_bytes);
+      }
+    };
+    uint4 keys_a[kRounds], values_a[kRounds], keys_b[kRounds], values_b[kRounds];
+    if (steps > 0) load(0, keys_a, values_a);
+    for (int j = 0; j < steps; j += 2) {
+      if (j + 1 < steps) load(j + 1, keys_b, values_b);
+      put(j, keys_a, values_a);
+      if (j + 1 < steps) {
+        if (j + 2 < steps) load(j + 2, keys_a, values_a);
+        put(j + 1, keys_b, values_b);
+      }
     }
   }
 
@@ -524,6 +606,13 @@ int32_t launch_tiles(const AttentionParams& p, cudaStream_t stream, char* messag
       cudaFuncSetAttribute(tile_kernel<T, D>, cudaFuncAttributePreferredSharedMemoryCarveout,
                            cudaSharedmemCarveoutMaxShared) != cudaSuccess) {
     return fail(NML_SM100_LAUNCH_FAILURE, "cannot configure shared memory", message, capacity);
+  }
+  // the shares above count on what the compiler gave every thread
+  cudaFuncAttributes attributes;
+  if (cudaFuncGetAttributes(&attributes, tile_kernel<T, D>) != cudaSuccess ||
+      attributes.numRegs != kLaunchRegisters) {
+    return fail(NML_SM100_LAUNCH_FAILURE, "tile kernel built with another register count", message,
+                capacity);
   }
   const int64_t items = query_tiles(p.tokens, p.cache.batch, p.group);
   tile_kernel<T, D><<<static_cast<unsigned>(items * p.splits * p.cache.kv_heads), kThreads,
