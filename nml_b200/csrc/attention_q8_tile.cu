@@ -72,7 +72,9 @@ template <int D>
 struct Control {
   uint64_t tiles_full[Shape<D>::kStages], tiles_free[Shape<D>::kStages];
   uint64_t scores_full[Shape<D>::kBuffers];
-  uint64_t query_full, weights_full, product_done, drained;
+  // one for each buffer: a warp may run ahead of the others by as many steps as there are buffers
+  uint64_t weights_full[Shape<D>::kBuffers], product_done[Shape<D>::kBuffers];
+  uint64_t query_full, drained;
   uint32_t tmem;
   int abort_flag;
   int sequence, tile;
@@ -120,7 +122,9 @@ tile_kernel(const AttentionParams p) {
   __shared__ __align__(16) Control<D> control;
   volatile int* const abort_flag = &control.abort_flag;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // through a shuffle: the compiler then knows the roles' branches and loops to be warp-uniform
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
   const int kv_head = blockIdx.x % p.cache.kv_heads;
   const int item = blockIdx.x / p.cache.kv_heads / p.splits;
   const int split = blockIdx.x / p.cache.kv_heads % p.splits;
@@ -160,10 +164,12 @@ tile_kernel(const AttentionParams p) {
       mbar_init(&control.tiles_full[i], kWidenThreads);
       mbar_init(&control.tiles_free[i], 1);
     }
-    for (int i = 0; i < S::kBuffers; ++i) mbar_init(&control.scores_full[i], 1);
+    for (int i = 0; i < S::kBuffers; ++i) {
+      mbar_init(&control.scores_full[i], 1);
+      mbar_init(&control.weights_full[i], kSoftmaxThreads);
+      mbar_init(&control.product_done[i], 1);
+    }
     mbar_init(&control.query_full, kSoftmaxThreads);
-    mbar_init(&control.weights_full, kSoftmaxThreads);
-    mbar_init(&control.product_done, 1);
     mbar_init(&control.drained, 1);
     control.abort_flag = 0;
     mbar_fence_init();
@@ -183,7 +189,7 @@ tile_kernel(const AttentionParams p) {
   const int all_steps = (v.pages + kStepPages - 1) / kStepPages;
   const int per_split = (all_steps + p.splits - 1) / p.splits;
   const int step_begin = min(all_steps, split * per_split);
-  const int steps = min(all_steps - step_begin, per_split);
+  const int steps = __shfl_sync(0xffffffffu, min(all_steps - step_begin, per_split), 0);
 
   if (warp == kMmaWarp) {
     tmem_alloc(&control.tmem, kTmemColumns);
@@ -192,11 +198,18 @@ tile_kernel(const AttentionParams p) {
   tcgen05_fence_before_sync();
   __syncthreads();
   tcgen05_fence_after_sync();
-  const uint32_t tmem = control.tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, control.tmem, 0);
 
   auto wait = [&](uint64_t* bar, int phase, int site) {
     mbar_wait_or_abort(bar, static_cast<uint32_t>(phase) & 1u, abort_flag, p.status, site);
     __syncwarp();
+  };
+
+  // The product of step j.  Whoever has step j's scores knows that the product kBuffers steps
+  // back is complete, and no product passes a step that this warp has not handed over: with a
+  // barrier for each buffer a parity names one phase only.
+  auto wait_product = [&](int j) {
+    wait(&control.product_done[j % S::kBuffers], j / S::kBuffers, kSiteProduct);
   };
 
   if (warp < kWidenWarp) {
@@ -260,6 +273,15 @@ tile_kernel(const AttentionParams p) {
       mbar_arrive(&control.query_full);
     }
 
+    // steps whose tokens every row of the tile sees: behind the last row's window start, in front
+    // of the first row's own token
+    const int last_start = p.window > 0 ? max(0, first_position + rows - p.window) : 0;
+    const int first_whole = last_start == 0 ? 0 : v.front + (last_start + kCachePage - 1) /
+                                                                kCachePage - v.back;
+    const int whole_pages = v.front + max(first_position + 1, 0) / kCachePage - v.back;
+    const int whole_begin = (first_whole + kStepPages - 1) / kStepPages - step_begin;
+    const int whole_end = max(whole_pages, 0) / kStepPages - step_begin;
+
     float running_max = -INFINITY, running_sum = 0.0f;
     for (int j = 0; j < steps; ++j) {
       const int buffer = j % S::kBuffers, stage = j % S::kStages;
@@ -279,32 +301,46 @@ tile_kernel(const AttentionParams p) {
         s[32 + i] = __uint_as_float(scores_hi[i]);
       }
       const uint4 nan_words = *reinterpret_cast<const uint4*>(control.any_nan[stage]);
-      bool whole = (nan_words.x | nan_words.y | nan_words.z | nan_words.w) == 0;
-#pragma unroll
-      for (int q = 0; q < kStepPages; ++q) {
-        const int t = control.pages[stage][q].token;
-        whole = whole && t + kCachePage <= length && (t >= start || t + kCachePage <= p.first);
-      }
-      if (!__all_sync(0xffffffffu, whole)) {
-#pragma unroll
+      const bool nans = (nan_words.x | nan_words.y | nan_words.z | nan_words.w) != 0;
+      if (j < whole_begin || j >= whole_end || nans) {
+        // bit i: token i of the step is seen, its value row is NaN; loops, so that the steps
+        // without masks branch over all of this
+        uint32_t seen[2] = {0, 0}, nan[2] = {0, 0};
+#pragma unroll 1
         for (int q = 0; q < kStepPages; ++q) {
           const int t = control.pages[stage][q].token;
-#pragma unroll
-          for (int i = 0; i < kCachePage; ++i) {
-            const bool seen = t + i < length && (t + i >= start || t + i < p.first);
-            const bool nan = control.row_nan[stage][q * kCachePage + i] != 0;
-            s[q * kCachePage + i] =
-                seen ? (nan ? __uint_as_float(0x7fc00000u) : s[q * kCachePage + i]) : -INFINITY;
+          auto below = [&](int limit) {  // bits of the page's tokens in front of `limit`
+            return (1u << min(max(limit - t, 0), kCachePage)) - 1u;
+          };
+          const uint32_t bits = below(length) & (~below(start) | below(p.first));
+          uint32_t nan_bits = 0;
+          if (nans) {
+#pragma unroll 1
+            for (int i = 0; i < kCachePage; ++i) {
+              nan_bits |= static_cast<uint32_t>(control.row_nan[stage][q * kCachePage + i]) << i;
+            }
           }
+          const int shift = q * kCachePage & 31;
+          seen[0] |= q < 2 ? bits << shift : 0u;
+          seen[1] |= q < 2 ? 0u : bits << shift;
+          nan[0] |= q < 2 ? nan_bits << shift : 0u;
+          nan[1] |= q < 2 ? 0u : nan_bits << shift;
+        }
+#pragma unroll
+        for (int i = 0; i < kStepTokens; ++i) {
+          if ((nan[i / 32] >> (i % 32) & 1u) != 0) s[i] = __uint_as_float(0x7fc00000u);
+          if ((seen[i / 32] >> (i % 32) & 1u) == 0) s[i] = -INFINITY;
         }
       }
       float page_factor[kStepPages];
       float top = -INFINITY;
 #pragma unroll
       for (int q = 0; q < kStepPages; ++q) {
-        float m = s[q * kCachePage];
+        float m = fmaxf(s[q * kCachePage], s[q * kCachePage + 1]);
 #pragma unroll
-        for (int i = 1; i < kCachePage; ++i) m = fmaxf(m, s[q * kCachePage + i]);
+        for (int i = 2; i < kCachePage; i += 2) {
+          m = fmaxf(fmaxf(m, s[q * kCachePage + i]), s[q * kCachePage + i + 1]);
+        }
         page_factor[q] = factor * control.pages[stage][q].key_scale;
         top = fmaxf(top, fmaf(m, page_factor[q], control.pages[stage][q].value_exponent));
       }
@@ -314,7 +350,7 @@ tile_kernel(const AttentionParams p) {
         const float next = raise ? top : running_max;
         const float rescale = raise ? exp2_fast(running_max - next) : 1.0f;
         if (j > 0) {
-          wait(&control.product_done, j - 1, kSiteProduct);
+          wait_product(j - 1);
           tcgen05_fence_after_sync();
 #pragma unroll
           for (int c = 0; c < D; c += 16) {
@@ -360,12 +396,12 @@ tile_kernel(const AttentionParams p) {
       }
       tmem_store_wait();
       tcgen05_fence_before_sync();
-      mbar_arrive(&control.weights_full);
+      mbar_arrive(&control.weights_full[buffer]);
     }
 
     // ---- the rows' results ----
     if (steps > 0) {
-      wait(&control.product_done, steps - 1, kSiteProduct);
+      wait_product(steps - 1);
       tcgen05_fence_after_sync();
     }
     const int64_t query_head = static_cast<int64_t>(first_row + token) * p.query_heads + head;
@@ -438,7 +474,7 @@ tile_kernel(const AttentionParams p) {
       }
       for (int j = 0; j < steps; ++j) {
         const int stage = j % S::kStages, buffer = j % S::kBuffers;
-        wait(&control.weights_full, j, kSiteWeights);
+        wait(&control.weights_full[buffer], j / S::kBuffers, kSiteWeights);
         tcgen05_fence_after_sync();
         const uint32_t values = smem_u32(shared + stage * 2 * S::kTileBytes + S::kTileBytes);
 #pragma unroll
@@ -450,10 +486,10 @@ tile_kernel(const AttentionParams p) {
                                 desc_hi | low, product_idesc, j > 0 || k > 0 ? 1u : 0u);
         }
         umma_commit_elect(&control.tiles_free[stage]);
-        umma_commit_elect(&control.product_done);
+        umma_commit_elect(&control.product_done[buffer]);
         if (j + S::kBuffers < steps) {
           // the scores go over the weights that this product reads
-          wait(&control.product_done, j, kSiteProduct);
+          wait_product(j);
           scores(j + S::kBuffers);
         }
       }
