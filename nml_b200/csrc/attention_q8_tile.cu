@@ -15,9 +15,10 @@
 //              O += W V (A: weights in tensor memory, B: values, MN-major: tokens are rows)
 // Registers move from the last two warpgroups to the softmax, which holds a row's 64 scores.
 //
-// The running maximum M only stabilises: weights reach up to 2^8 before it is raised (F16 holds
-// them, sums are f32), so the accumulator in tensor memory is rescaled a few times for a row and
-// not at every step.  A value row of NaN codes (stored whole by the append) becomes zeros in the
+// The running maximum M only stabilises: weights above one are as good as those below as long as
+// F16 holds them (sums are f32).  So a step is weighted against the maximum of the steps before it,
+// and only when a page's weights sum to more than 2^14 is its own maximum formed, the accumulator
+// in tensor memory rescaled and the step repeated: once or twice for a row.  A value row of NaN codes (stored whole by the append) becomes zeros in the
 // product and NaN scores for the rows that see it, so that it does not reach the rows that do not.
 //
 // What bounds it: one exponential for each score.  A step of 128 x 64 takes 512 clocks of the SM's
@@ -38,7 +39,8 @@ constexpr int kWidenWarp = 4;
 constexpr int kMmaWarp = 8;
 constexpr int kThreads = 384;  // the last three warps only give their registers
 constexpr int kLaunchRegisters = 80;  // of a thread: two CTAs fill an SM
-constexpr float kSlack = 8.0f;  // log2 of the largest weight before the maximum is raised
+// Sum of a page's 16 weights up to which the maximum so far still serves: F16 holds each of them.
+constexpr float kLargestSum = 16384.0f;
 constexpr int kTmemColumns = 256;
 
 // Bits 8 + site of the status word say which wait ran out.
@@ -286,113 +288,135 @@ tile_kernel(const AttentionParams p) {
     for (int j = 0; j < steps; ++j) {
       const int buffer = j % S::kBuffers, stage = j % S::kStages;
       const uint32_t columns = lanes + S::kScores + buffer * kStepTokens;
-      wait(&control.scores_full[buffer], j / S::kBuffers, kSiteScores);
-      tcgen05_fence_after_sync();
-      // long complete; orders the reads of the stage's page data behind their writes
-      wait(&control.tiles_full[stage], j / S::kStages, kSiteTiles);
-      uint32_t scores_lo[32], scores_hi[32];
-      tmem_load_32x32(columns, scores_lo);
-      tmem_load_32x32(columns + 32, scores_hi);
-      tmem_load_wait();
-      float s[kStepTokens];
+      wait(&control.tiles_full[stage], j / S::kStages, kSiteTiles);  // for the page data
+      float page_factor[kStepPages], value_exponent[kStepPages], unscale[kStepPages];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        s[i] = __uint_as_float(scores_lo[i]);
-        s[32 + i] = __uint_as_float(scores_hi[i]);
+      for (int q = 0; q < kStepPages; ++q) {
+        const float4 info = *reinterpret_cast<const float4*>(&control.pages[stage][q]);
+        page_factor[q] = factor * info.x;
+        value_exponent[q] = info.y;
+        unscale[q] = info.z;
       }
       const uint4 nan_words = *reinterpret_cast<const uint4*>(control.any_nan[stage]);
       const bool nans = (nan_words.x | nan_words.y | nan_words.z | nan_words.w) != 0;
-      if (j < whole_begin || j >= whole_end || nans) {
-        // bit i: token i of the step is seen, its value row is NaN; loops, so that the steps
-        // without masks branch over all of this
-        uint32_t seen[2] = {0, 0}, nan[2] = {0, 0};
+      wait(&control.scores_full[buffer], j / S::kBuffers, kSiteScores);
+      tcgen05_fence_after_sync();
+
+      // Weights against the maximum so far; their sum tells whether it still serves.  Only when it
+      // does not (or there is none yet) is the step's maximum formed and the step done again.
+      uint32_t packed[kStepTokens / 2];
+      float step_sum;
+      bool with_maximum = __any_sync(0xffffffffu, running_max == -INFINITY);
+      while (true) {
+        uint32_t scores_lo[32], scores_hi[32];
+        tmem_load_32x32(columns, scores_lo);
+        tmem_load_32x32(columns + 32, scores_hi);
+        tmem_load_wait();
+        float s[kStepTokens];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          s[i] = __uint_as_float(scores_lo[i]);
+          s[32 + i] = __uint_as_float(scores_hi[i]);
+        }
+        if (j < whole_begin || j >= whole_end || nans) {
+          // bit i: token i of the step is seen, its value row is NaN; loops, so that the steps
+          // without masks branch over all of this
+          uint32_t seen[2] = {0, 0}, nan[2] = {0, 0};
 #pragma unroll 1
+          for (int q = 0; q < kStepPages; ++q) {
+            const int t = control.pages[stage][q].token;
+            auto below = [&](int limit) {  // bits of the page's tokens in front of `limit`
+              return (1u << min(max(limit - t, 0), kCachePage)) - 1u;
+            };
+            const uint32_t bits = below(length) & (~below(start) | below(p.first));
+            uint32_t nan_bits = 0;
+            if (nans) {
+#pragma unroll 1
+              for (int i = 0; i < kCachePage; ++i) {
+                nan_bits |= static_cast<uint32_t>(control.row_nan[stage][q * kCachePage + i]) << i;
+              }
+            }
+            const int shift = q * kCachePage & 31;
+            seen[0] |= q < 2 ? bits << shift : 0u;
+            seen[1] |= q < 2 ? 0u : bits << shift;
+            nan[0] |= q < 2 ? nan_bits << shift : 0u;
+            nan[1] |= q < 2 ? 0u : nan_bits << shift;
+          }
+#pragma unroll
+          for (int i = 0; i < kStepTokens; ++i) {
+            if ((nan[i / 32] >> (i % 32) & 1u) != 0) s[i] = __uint_as_float(0x7fc00000u);
+            if ((seen[i / 32] >> (i % 32) & 1u) == 0) s[i] = -INFINITY;
+          }
+        }
+        if (with_maximum) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int q = 0; q < kStepPages; ++q) {
+            float m = fmaxf(s[q * kCachePage], s[q * kCachePage + 1]);
+#pragma unroll
+            for (int i = 2; i < kCachePage; i += 2) {
+              m = fmaxf(fmaxf(m, s[q * kCachePage + i]), s[q * kCachePage + i + 1]);
+            }
+            top = fmaxf(top, fmaf(m, page_factor[q], value_exponent[q]));
+          }
+          const bool raise = top > running_max;  // also from -infinity
+          const float next = raise ? top : running_max;
+          const float rescale = raise ? exp2_fast(running_max - next) : 1.0f;
+          if (j > 0) {
+            wait_product(j - 1);
+            tcgen05_fence_after_sync();
+#pragma unroll
+            for (int c = 0; c < D; c += 16) {
+              uint32_t x[16], y[8], z[8];
+              tmem_load_32x16(lanes + S::kOut + c, x);
+              tmem_load_wait();
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                y[i] = __float_as_uint(__uint_as_float(x[i]) * rescale);
+                z[i] = __float_as_uint(__uint_as_float(x[i + 8]) * rescale);
+              }
+              tmem_store_32x8(lanes + S::kOut + c, y);
+              tmem_store_32x8(lanes + S::kOut + c + 8, z);
+            }
+          }
+          running_sum *= rescale;
+          running_max = next;
+        }
+        const float base = running_max == -INFINITY ? 0.0f : running_max;
+        step_sum = 0.0f;
+        float largest_sum = 0.0f;
+#pragma unroll
         for (int q = 0; q < kStepPages; ++q) {
-          const int t = control.pages[stage][q].token;
-          auto below = [&](int limit) {  // bits of the page's tokens in front of `limit`
-            return (1u << min(max(limit - t, 0), kCachePage)) - 1u;
-          };
-          const uint32_t bits = below(length) & (~below(start) | below(p.first));
-          uint32_t nan_bits = 0;
-          if (nans) {
-#pragma unroll 1
-            for (int i = 0; i < kCachePage; ++i) {
-              nan_bits |= static_cast<uint32_t>(control.row_nan[stage][q * kCachePage + i]) << i;
-            }
-          }
-          const int shift = q * kCachePage & 31;
-          seen[0] |= q < 2 ? bits << shift : 0u;
-          seen[1] |= q < 2 ? 0u : bits << shift;
-          nan[0] |= q < 2 ? nan_bits << shift : 0u;
-          nan[1] |= q < 2 ? 0u : nan_bits << shift;
-        }
+          const float offset = value_exponent[q] - base;
+          const uint64_t factor2 = pack_f32x2(page_factor[q], page_factor[q]);
+          const uint64_t offset2 = pack_f32x2(offset, offset);
+          uint64_t sum2 = 0;
 #pragma unroll
-        for (int i = 0; i < kStepTokens; ++i) {
-          if ((nan[i / 32] >> (i % 32) & 1u) != 0) s[i] = __uint_as_float(0x7fc00000u);
-          if ((seen[i / 32] >> (i % 32) & 1u) == 0) s[i] = -INFINITY;
+          for (int i = 0; i < 8; ++i) {
+            float a, b;
+            unpack_f32x2(fma_f32x2(pack_f32x2(s[q * kCachePage + 2 * i],
+                                              s[q * kCachePage + 2 * i + 1]),
+                                   factor2, offset2),
+                         a, b);
+            a = exp2_fast(a);
+            b = exp2_fast(b);
+            sum2 = add_f32x2(sum2, pack_f32x2(a, b));
+            packed[8 * q + i] = Elem<__half>::pack2(a, b);
+          }
+          float sum_even, sum_odd;
+          unpack_f32x2(sum2, sum_even, sum_odd);
+          const float sum = sum_even + sum_odd;
+          largest_sum = fmaxf(largest_sum, sum);
+          step_sum = fmaf(sum, unscale[q], step_sum);
         }
+        if (with_maximum || !__any_sync(0xffffffffu, largest_sum > kLargestSum)) break;
+        with_maximum = true;
       }
-      float page_factor[kStepPages];
-      float top = -INFINITY;
+      running_sum += step_sum;
 #pragma unroll
       for (int q = 0; q < kStepPages; ++q) {
-        float m = fmaxf(s[q * kCachePage], s[q * kCachePage + 1]);
-#pragma unroll
-        for (int i = 2; i < kCachePage; i += 2) {
-          m = fmaxf(fmaxf(m, s[q * kCachePage + i]), s[q * kCachePage + i + 1]);
-        }
-        page_factor[q] = factor * control.pages[stage][q].key_scale;
-        top = fmaxf(top, fmaf(m, page_factor[q], control.pages[stage][q].value_exponent));
-      }
-      // raise the maximum only when the weights would leave F16's comfortable range
-      const bool raise = top > running_max + kSlack;  // also from -infinity
-      if (__any_sync(0xffffffffu, raise)) {
-        const float next = raise ? top : running_max;
-        const float rescale = raise ? exp2_fast(running_max - next) : 1.0f;
-        if (j > 0) {
-          wait_product(j - 1);
-          tcgen05_fence_after_sync();
-#pragma unroll
-          for (int c = 0; c < D; c += 16) {
-            uint32_t x[16], y[8], z[8];
-            tmem_load_32x16(lanes + S::kOut + c, x);
-            tmem_load_wait();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              y[i] = __float_as_uint(__uint_as_float(x[i]) * rescale);
-              z[i] = __float_as_uint(__uint_as_float(x[i + 8]) * rescale);
-            }
-            tmem_store_32x8(lanes + S::kOut + c, y);
-            tmem_store_32x8(lanes + S::kOut + c + 8, z);
-          }
-        }
-        running_sum *= rescale;
-        running_max = next;
-      }
-      const float base = running_max == -INFINITY ? 0.0f : running_max;
-#pragma unroll
-      for (int q = 0; q < kStepPages; ++q) {
-        const float offset = control.pages[stage][q].value_exponent - base;
-        const uint64_t factor2 = pack_f32x2(page_factor[q], page_factor[q]);
-        const uint64_t offset2 = pack_f32x2(offset, offset);
-        uint32_t packed[8];
-        uint64_t sum2 = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float a, b;
-          unpack_f32x2(fma_f32x2(pack_f32x2(s[q * kCachePage + 2 * i],
-                                            s[q * kCachePage + 2 * i + 1]),
-                                 factor2, offset2),
-                       a, b);
-          a = exp2_fast(a);
-          b = exp2_fast(b);
-          sum2 = add_f32x2(sum2, pack_f32x2(a, b));
-          packed[i] = Elem<__half>::pack2(a, b);
-        }
-        float sum_even, sum_odd;
-        unpack_f32x2(sum2, sum_even, sum_odd);
-        running_sum = fmaf(sum_even + sum_odd, control.pages[stage][q].unscale, running_sum);
-        tmem_store_32x8(columns + 8 * q, packed);
+        const uint32_t(&page)[8] = *reinterpret_cast<const uint32_t(*)[8]>(&packed[8 * q]);
+        tmem_store_32x8(columns + 8 * q, page);
       }
       tmem_store_wait();
       tcgen05_fence_before_sync();
