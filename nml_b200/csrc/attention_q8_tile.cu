@@ -8,18 +8,20 @@
 //   warps 0-3  softmax, one thread for each row: q into tensor memory (F16, a power of two for the
 //              row), then for every step the scores out of tensor memory, maximum, weights back
 //              into tensor memory over the scores; rescales the accumulator when needed
-//   warps 4-7  widen the codes: 16-byte loads, E4M3 to F16 (exact, the block scales stay out),
-//              128-byte swizzled stores; the next step's loads are in flight meanwhile, page
-//              table entries and scales are fetched for 32 pages at a time, 32 pages ahead
+//   warps 4-7  widen the codes: E4M3 to F16 (exact, the block scales stay out), from where they are
+//              staged into 128-byte swizzled tiles
 //   warp 8     issues the products: S = Q K^T (A: q in tensor memory, B: keys, K-major) and
 //              O += W V (A: weights in tensor memory, B: values, MN-major: tokens are rows)
+//   warp 9     brings in the blocks of codes by bulk copies some steps ahead; page table entries
+//              and scales are fetched for 32 pages at a time, 32 pages ahead
 // Registers move from the last two warpgroups to the softmax, which holds a row's 64 scores.
 //
 // The running maximum M only stabilises: weights above one are as good as those below as long as
 // F16 holds them (sums are f32).  So a step is weighted against the maximum of the steps before it,
 // and only when a page's weights sum to more than 2^14 is its own maximum formed, the accumulator
-// in tensor memory rescaled and the step repeated: once or twice for a row.  A value row of NaN codes (stored whole by the append) becomes zeros in the
-// product and NaN scores for the rows that see it, so that it does not reach the rows that do not.
+// in tensor memory rescaled and the step repeated: once or twice for a row.  A key or value row of
+// NaN codes (stored whole by the append) enters the products as zeros and marks the rows that see
+// it, whose results become NaN; it does not reach the rows that do not.
 //
 // What bounds it: one exponential for each score.  A step of 128 x 64 takes 512 clocks of the SM's
 // 16 exponentials per clock and 256 (head_dim 64) of the tensor cores.
@@ -35,9 +37,8 @@ constexpr int kStepTokens = 64;
 constexpr int kStepPages = kStepTokens / kCachePage;
 constexpr int kSoftmaxThreads = 128;
 constexpr int kWidenThreads = 128;
-constexpr int kWidenWarp = 4;
-constexpr int kMmaWarp = 8;
-constexpr int kThreads = 384;  // the last three warps only give their registers
+constexpr int kWidenWarp = 4, kMmaWarp = 8, kLoadWarp = 9;
+constexpr int kThreads = 384;  // the last two warps only give their registers
 constexpr int kLaunchRegisters = 80;  // of a thread: two CTAs fill an SM
 // Sum of a page's 16 weights up to which the maximum so far still serves: F16 holds each of them.
 constexpr float kLargestSum = 16384.0f;
@@ -45,7 +46,7 @@ constexpr int kTmemColumns = 256;
 
 // Bits 8 + site of the status word say which wait ran out.
 constexpr int kSiteScores = 16, kSiteWeights = 17, kSiteTiles = 18, kSiteProduct = 19,
-              kSiteFree = 20;
+              kSiteFree = 20, kSiteStaged = 21;
 
 // What the softmax needs to know of a page: score factor, exponent of the values, its inverse
 // power for the denominator, first token.
@@ -57,21 +58,29 @@ struct alignas(16) PageInfo {
 template <int D>
 struct Shape {
   static constexpr int kTileBytes = kStepTokens * D * 2;
-  static constexpr int kStages = D == 64 ? 4 : 3;
+  static constexpr int kStages = D == 64 ? 3 : 2;       // F16 tiles
+  static constexpr int kCodeBytes = kStepTokens * D;    // of a step's keys, then of its values
+  static constexpr int kStaged = D == 64 ? 6 : 2;       // steps of codes on their way
   static constexpr int kBuffers = D == 64 ? 2 : 1;  // score buffers in tensor memory
   static constexpr int kOut = 0, kQuery = D, kScores = D + D / 2;
-  static constexpr int kSharedBytes = kStages * 2 * kTileBytes + 1024;
+  static constexpr int kStagedOffset = kStages * 2 * kTileBytes;
+  static constexpr int kSharedBytes = kStagedOffset + kStaged * 2 * kCodeBytes + 1024;
   // The three warpgroups' shares of the CTA's registers at launch.
-  static constexpr int kSoftmaxRegisters = D == 64 ? 144 : 136;
-  static constexpr int kWidenRegisters = D == 64 ? 72 : 80;
-  static constexpr int kMmaRegisters = 24;
+  static constexpr int kSoftmaxRegisters = D == 64 ? 144 : 128;
+  static constexpr int kWidenRegisters = D == 64 ? 56 : 72;
+  static constexpr int kMmaRegisters = 40;
   static_assert(kSoftmaxRegisters + kWidenRegisters + kMmaRegisters == 3 * kLaunchRegisters,
                 "a share that the launch does not cover would be waited for without end");
+  static_assert(kStaged + kStages < 16, "page data");
   static_assert(kScores + kBuffers * kStepTokens <= kTmemColumns, "tensor memory");
 };
 
+// Steps whose page data is kept: more than the staged and the widened ones together.
+constexpr int kInfoSteps = 16;
+
 template <int D>
 struct Control {
+  uint64_t staged_full[Shape<D>::kStaged], staged_free[Shape<D>::kStaged];
   uint64_t tiles_full[Shape<D>::kStages], tiles_free[Shape<D>::kStages];
   uint64_t scores_full[Shape<D>::kBuffers];
   // one for each buffer: a warp may run ahead of the others by as many steps as there are buffers
@@ -80,18 +89,19 @@ struct Control {
   uint32_t tmem;
   int abort_flag;
   int sequence, tile;
-  PageInfo pages[Shape<D>::kStages][kStepPages];
+  PageInfo pages[kInfoSteps][kStepPages];
   alignas(16) uint32_t any_nan[Shape<D>::kStages][4];  // read 16 bytes at a time
   uint8_t row_nan[Shape<D>::kStages][kStepTokens];
 };
 
+// The warpgroup's share of the CTA's registers; a larger one waits for others to give theirs.
 template <int N>
-__device__ __forceinline__ void more_registers() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void fewer_registers() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+__device__ __forceinline__ void take_registers() {
+  if constexpr (N > kLaunchRegisters) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+  }
 }
 
 // Two f32 at a time.
@@ -162,6 +172,10 @@ tile_kernel(const AttentionParams p) {
     }
   }
   if (threadIdx.x == kMmaWarp * 32) {
+    for (int i = 0; i < S::kStaged; ++i) {
+      mbar_init(&control.staged_full[i], 1);
+      mbar_init(&control.staged_free[i], kWidenThreads);
+    }
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(&control.tiles_full[i], kWidenThreads);
       mbar_init(&control.tiles_free[i], 1);
@@ -216,7 +230,7 @@ tile_kernel(const AttentionParams p) {
 
   if (warp < kWidenWarp) {
     // ------------------------------------------------------------------ softmax
-    more_registers<S::kSoftmaxRegisters>();
+    take_registers<S::kSoftmaxRegisters>();
     const int row = threadIdx.x;
     const int token = row / p.group;
     const int head = kv_head * p.group + row - token * p.group;
@@ -228,25 +242,27 @@ tile_kernel(const AttentionParams p) {
 
     // q: largest magnitude, then F16 into tensor memory, column c holding elements 2c and 2c + 1
     float factor = p.scale_log2;
+    bool poisoned;  // something the row sees, or the row itself, is NaN: so is its result
     {
       const T* source = static_cast<const T*>(p.query) +
                         static_cast<int64_t>(first_row + token) * p.query_token_stride +
                         head * p.query_head_stride;
-      uint32_t largest = 0;
-      if constexpr (!std::is_same<T, __half>::value) {
-        if (live) {
+      uint32_t largest = 0;  // magnitude bits in the upper half
+      if (live) {
 #pragma unroll
-          for (int i = 0; i < D / 8; ++i) {
-            const uint4 x = reinterpret_cast<const uint4*>(source)[i];
-            const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+        for (int i = 0; i < D / 8; ++i) {
+          const uint4 x = reinterpret_cast<const uint4*>(source)[i];
+          const uint32_t words[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              largest = max(largest, max((words[w] & 0x7fffu) << 16, words[w] & 0x7fff0000u));
-            }
+          for (int w = 0; w < 4; ++w) {
+            largest = max(largest, max((words[w] & 0x7fffu) << 16, words[w] & 0x7fff0000u));
           }
         }
       }
-      const int shift = std::is_same<T, __half>::value ? 0 : query_shift(largest);
+      // a query with an infinity or a NaN gives NaN; its scores need not be formed
+      constexpr bool kHalf = std::is_same<T, __half>::value;
+      poisoned = largest >= (kHalf ? 0x7c000000u : 0x7f800000u);
+      const int shift = kHalf ? 0 : query_shift(largest);
       const float up = exp2_int(shift);
       factor *= exp2_int(-shift);
 #pragma unroll
@@ -255,11 +271,11 @@ tile_kernel(const AttentionParams p) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint4 x = make_uint4(0, 0, 0, 0);
-          if (live) x = reinterpret_cast<const uint4*>(source)[2 * i + h];
+          if (live && !poisoned) x = reinterpret_cast<const uint4*>(source)[2 * i + h];
           const uint32_t words[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            if constexpr (std::is_same<T, __half>::value) {
+            if constexpr (kHalf) {
               packed[4 * h + w] = words[w];
             } else {
               packed[4 * h + w] = Elem<__half>::pack2(Elem<T>::from_bits(words[w] & 0xffffu) * up,
@@ -288,11 +304,12 @@ tile_kernel(const AttentionParams p) {
     for (int j = 0; j < steps; ++j) {
       const int buffer = j % S::kBuffers, stage = j % S::kStages;
       const uint32_t columns = lanes + S::kScores + buffer * kStepTokens;
+      const PageInfo* const pages = control.pages[j % kInfoSteps];
       wait(&control.tiles_full[stage], j / S::kStages, kSiteTiles);  // for the page data
       float page_factor[kStepPages], value_exponent[kStepPages], unscale[kStepPages];
 #pragma unroll
       for (int q = 0; q < kStepPages; ++q) {
-        const float4 info = *reinterpret_cast<const float4*>(&control.pages[stage][q]);
+        const float4 info = *reinterpret_cast<const float4*>(&pages[q]);
         page_factor[q] = factor * info.x;
         value_exponent[q] = info.y;
         unscale[q] = info.z;
@@ -308,45 +325,39 @@ tile_kernel(const AttentionParams p) {
       float step_sum;
       bool with_maximum = __any_sync(0xffffffffu, running_max == -INFINITY);
       while (true) {
-        uint32_t scores_lo[32], scores_hi[32];
-        tmem_load_32x32(columns, scores_lo);
-        tmem_load_32x32(columns + 32, scores_hi);
+        uint32_t scores[2][32];
+        tmem_load_32x32(columns, scores[0]);
+        tmem_load_32x32(columns + 32, scores[1]);
         tmem_load_wait();
         float s[kStepTokens];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          s[i] = __uint_as_float(scores_lo[i]);
-          s[32 + i] = __uint_as_float(scores_hi[i]);
-        }
+        for (int i = 0; i < kStepTokens; ++i) s[i] = __uint_as_float(scores[i / 32][i % 32]);
         if (j < whole_begin || j >= whole_end || nans) {
-          // bit i: token i of the step is seen, its value row is NaN; loops, so that the steps
-          // without masks branch over all of this
-          uint32_t seen[2] = {0, 0}, nan[2] = {0, 0};
+          // bit i: token i is seen; loops, so that the steps without masks branch over all of this
+          uint32_t seen[2] = {0, 0};
 #pragma unroll 1
           for (int q = 0; q < kStepPages; ++q) {
-            const int t = control.pages[stage][q].token;
+            const int t = pages[q].token;
             auto below = [&](int limit) {  // bits of the page's tokens in front of `limit`
               return (1u << min(max(limit - t, 0), kCachePage)) - 1u;
             };
             const uint32_t bits = below(length) & (~below(start) | below(p.first));
-            uint32_t nan_bits = 0;
             if (nans) {
+              const uint8_t* const row_nan = &control.row_nan[stage][q * kCachePage];
 #pragma unroll 1
               for (int i = 0; i < kCachePage; ++i) {
-                nan_bits |= static_cast<uint32_t>(control.row_nan[stage][q * kCachePage + i]) << i;
+                if (row_nan[i] != 0 && (bits >> i & 1u) != 0) poisoned = true;
               }
             }
             const int shift = q * kCachePage & 31;
             seen[0] |= q < 2 ? bits << shift : 0u;
             seen[1] |= q < 2 ? 0u : bits << shift;
-            nan[0] |= q < 2 ? nan_bits << shift : 0u;
-            nan[1] |= q < 2 ? 0u : nan_bits << shift;
           }
 #pragma unroll
           for (int i = 0; i < kStepTokens; ++i) {
-            if ((nan[i / 32] >> (i % 32) & 1u) != 0) s[i] = __uint_as_float(0x7fc00000u);
             if ((seen[i / 32] >> (i % 32) & 1u) == 0) s[i] = -INFINITY;
           }
+          __syncwarp();
         }
         if (with_maximum) {
           float top = -INFINITY;
@@ -367,16 +378,17 @@ tile_kernel(const AttentionParams p) {
             tcgen05_fence_after_sync();
 #pragma unroll
             for (int c = 0; c < D; c += 16) {
+              const uint32_t out_columns = lanes + S::kOut + c;
               uint32_t x[16], y[8], z[8];
-              tmem_load_32x16(lanes + S::kOut + c, x);
+              tmem_load_32x16(out_columns, x);
               tmem_load_wait();
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
                 y[i] = __float_as_uint(__uint_as_float(x[i]) * rescale);
                 z[i] = __float_as_uint(__uint_as_float(x[i + 8]) * rescale);
               }
-              tmem_store_32x8(lanes + S::kOut + c, y);
-              tmem_store_32x8(lanes + S::kOut + c + 8, z);
+              tmem_store_32x8(out_columns, y);
+              tmem_store_32x8(out_columns + 8, z);
             }
           }
           running_sum *= rescale;
@@ -413,6 +425,7 @@ tile_kernel(const AttentionParams p) {
         with_maximum = true;
       }
       running_sum += step_sum;
+      // over the thread's own scores
 #pragma unroll
       for (int q = 0; q < kStepPages; ++q) {
         const uint32_t(&page)[8] = *reinterpret_cast<const uint32_t(*)[8]>(&packed[8 * q]);
@@ -429,11 +442,13 @@ tile_kernel(const AttentionParams p) {
       tcgen05_fence_after_sync();
     }
     const int64_t query_head = static_cast<int64_t>(first_row + token) * p.query_heads + head;
+    // a row that sees nothing has no maximum; its output is zero
+    if (running_max == -INFINITY) running_sum = 0.0f;
+    if (poisoned) running_sum = __uint_as_float(0x7fc00000u);
     float denominator = running_sum;
     if (p.sinks != nullptr && live) {
       denominator += exp2f(p.sinks[head] * kLog2e - running_max);
     }
-    // only a row that sees nothing has a sum of exactly zero; its output is zero
     const float inverse = running_sum == 0.0f ? 0.0f : 1.0f / denominator;
     float* partial = p.partial + (query_head * p.splits + split) * (D + 2);
     T* out = static_cast<T*>(p.output) + query_head * D;
@@ -471,8 +486,78 @@ tile_kernel(const AttentionParams p) {
     }
   } else if (warp >= kMmaWarp) {
     // ------------------------------------------------------------------ matrix products
-    fewer_registers<S::kMmaRegisters>();
-    if (warp == kMmaWarp) {
+    take_registers<S::kMmaRegisters>();
+    if (warp == kLoadWarp) {
+      // Blocks of codes are contiguous: one bulk copy each.  Lane i holds page (-1: nothing there)
+      // and scale bytes of entry i of a group of 32 pages, the next group's beside them.
+      constexpr int kGroup = 32, kSteps = kGroup / kStepPages;
+      constexpr uint32_t kBlockBytes = kCachePage * D;
+      auto look_up = [&](int group, int& page, uint32_t& key_byte, uint32_t& value_byte) {
+        page = -1;
+        key_byte = value_byte = 0;
+        const int i = group * kGroup + lane;
+        if (i >= step_begin * kStepPages && i < min(v.pages, (step_begin + steps) * kStepPages)) {
+          page = physical_page(p.cache, sequence, i < v.front ? i : i - v.front + v.back,
+                               p.status);
+          if (page >= 0) {
+            const int64_t block = static_cast<int64_t>(page) * p.cache.kv_heads + kv_head;
+            key_byte = p.cache.scales[0][block];
+            value_byte = p.cache.scales[1][block];
+          }
+        }
+      };
+      int group = step_begin / kSteps;
+      int page, next_page;
+      uint32_t key_byte, value_byte, next_key, next_value;
+      look_up(group, page, key_byte, value_byte);
+      look_up(group + 1, next_page, next_key, next_value);
+      for (int j = 0; j < steps; ++j) {
+        const int step = step_begin + j, slot = j % S::kStaged;
+        if (j >= S::kStaged) wait(&control.staged_free[slot], j / S::kStaged - 1, kSiteFree);
+        const int at = step % kSteps * kStepPages + (lane & (kStepPages - 1));
+        const int held = __shfl_sync(0xffffffffu, page, at);
+        const uint32_t key_scale = __shfl_sync(0xffffffffu, key_byte, at);
+        const uint32_t value_scale = __shfl_sync(0xffffffffu, value_byte, at);
+        const bool mine = lane < kStepPages;
+        if (mine) {
+          // a page of nobody gives weights of zero and asks for no masks
+          PageInfo info{0.0f, -INFINITY, 0.0f, -kStepTokens};
+          if (held >= 0) {
+            const int i = step * kStepPages + lane;
+            const int e = scale_exponent(value_scale);
+            info = PageInfo{exp2_int(scale_exponent(key_scale)), static_cast<float>(e),
+                            exp2_int(-e), (i < v.front ? i : i - v.front + v.back) * kCachePage};
+          }
+          control.pages[j % kInfoSteps][lane] = info;
+        }
+        const uint32_t there = __ballot_sync(0xffffffffu, mine && held >= 0);
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&control.staged_full[slot], __popc(there) * 2 * kBlockBytes);
+        }
+        __syncwarp();
+        if (mine && held >= 0) {
+          const int64_t block = static_cast<int64_t>(held) * p.cache.kv_heads + kv_head;
+          uint8_t* const codes =
+              shared + S::kStagedOffset + slot * 2 * S::kCodeBytes + lane * kBlockBytes;
+          bulk_load(codes, p.cache.codes[0] + block * kBlockBytes, kBlockBytes,
+                    &control.staged_full[slot]);
+          bulk_load(codes + S::kCodeBytes, p.cache.codes[1] + block * kBlockBytes, kBlockBytes,
+                    &control.staged_full[slot]);
+        }
+        __syncwarp();
+        if ((step + 1) % kSteps == 0) {  // on to the next group of pages
+          ++group;
+          page = next_page;
+          key_byte = next_key;
+          value_byte = next_value;
+          look_up(group + 1, next_page, next_key, next_value);
+        }
+      }
+      // whatever has happened, no copy may land after the CTA is gone
+      for (int j = max(0, steps - S::kStaged); j < steps; ++j) {
+        mbar_wait(&control.staged_full[j % S::kStaged], j / S::kStaged & 1);
+      }
+    } else if (warp == kMmaWarp) {
       constexpr uint64_t desc_hi = static_cast<uint64_t>(kUmmaDescHiSw128) << 32;
       constexpr uint32_t score_idesc = umma_idesc_f16(kUmmaF16, kUmmaF16, kTileRows, kStepTokens);
       constexpr uint32_t product_idesc =
@@ -506,8 +591,9 @@ tile_kernel(const AttentionParams p) {
           // 16 tokens are 2 KB of 128-byte rows; the leading offset is the next 64 dimensions' tile
           const uint32_t address = values + k * 2048;
           const uint32_t low = ((address & 0x3ffffu) >> 4) | ((kStepTokens * 128 >> 4) << 16);
-          umma_f16_tmem_a_elect(tmem + S::kOut, tmem + S::kScores + buffer * kStepTokens + 8 * k,
-                                desc_hi | low, product_idesc, j > 0 || k > 0 ? 1u : 0u);
+          const uint32_t weights = tmem + S::kScores + buffer * kStepTokens + 8 * k;
+          umma_f16_tmem_a_elect(tmem + S::kOut, weights, desc_hi | low, product_idesc,
+                                j > 0 || k > 0 ? 1u : 0u);
         }
         umma_commit_elect(&control.tiles_free[stage]);
         umma_commit_elect(&control.product_done[buffer]);
@@ -525,126 +611,60 @@ tile_kernel(const AttentionParams p) {
     }
   } else {
     // ------------------------------------------------------------------ codes to F16 tiles
-    fewer_registers<S::kWidenRegisters>();
+    take_registers<S::kWidenRegisters>();
     constexpr int kParts = D / 16;                          // pieces of 16 codes of a token's row
-    constexpr int kTokens = kWidenThreads / kParts;         // tokens of one load of the group
-    constexpr int kRounds = kStepTokens / kTokens;          // loads for the keys of a step
-    constexpr int kGroup = 32;                              // pages looked up at once
+    constexpr int kTokens = kWidenThreads / kParts;         // tokens of one pass of the group
+    constexpr int kRounds = kStepTokens / kTokens;
     const int thread = threadIdx.x - kWidenWarp * 32;
     const int part = thread % kParts, first_token = thread / kParts;
-    // page of round r's token: r * (kTokens / 16) + lane_page
-    const int lane_page = first_token / kCachePage;
-    const uint32_t head_bytes = kCachePage * D;
-    const int64_t page_bytes = static_cast<int64_t>(p.cache.kv_heads) * head_bytes;
-    const int64_t thread_bytes = static_cast<int64_t>(kv_head) * head_bytes +
-                                 (first_token % kCachePage) * D + part * 16;
-    const uint8_t* const key_codes = p.cache.codes[0] + thread_bytes;
-    const uint8_t* const value_codes = p.cache.codes[1] + thread_bytes;
+    const int first_page = first_token / kCachePage;
+    const uint8_t* const own_codes = shared + S::kStagedOffset + thread * 16;
     uint8_t* const own_tile = shared + (part / 4) * (kStepTokens * 128) + first_token * 128;
     // 16-byte chunks 2 part and 2 part + 1 of a 128-byte row, swizzled by the token
     const int chunk_lo = ((2 * (part % 4)) ^ (first_token & 7)) * 16;
     const int chunk_hi = ((2 * (part % 4) + 1) ^ (first_token & 7)) * 16;
-
-    // lane i holds page (-1: nothing there) and scale bytes of entry i of a group of 32
-    auto look_up = [&](int group, int& page, uint32_t& bytes) {
-      page = -1;
-      bytes = 0;
-      const int i = group * kGroup + lane;
-      if (i >= step_begin * kStepPages && i < min(v.pages, (step_begin + steps) * kStepPages)) {
-        page = physical_page(p.cache, sequence, i < v.front ? i : i - v.front + v.back, p.status);
-        if (page >= 0) {
-          const int64_t block = static_cast<int64_t>(page) * p.cache.kv_heads + kv_head;
-          bytes = p.cache.scales[0][block] | static_cast<uint32_t>(p.cache.scales[1][block]) << 8;
-        }
-      }
-    };
-    constexpr int kSteps = kGroup / kStepPages;  // steps of a group of pages
-    int group = step_begin / kSteps;
-    int page, next_page;          // of this group and of the one behind it
-    uint32_t bytes, next_bytes;
-    look_up(group, page, bytes);
-    look_up(group + 1, next_page, next_bytes);
-
-    auto load = [&](int j, uint4 (&keys)[kRounds], uint4 (&values)[kRounds]) {
-      const int step = step_begin + j;
-      const int held = step / kSteps == group ? page : next_page;
-      const int at = step % kSteps * kStepPages + lane_page;
-#pragma unroll
-      for (int r = 0; r < kRounds; ++r) {
-        const int q = __shfl_sync(0xffffffffu, held, at + r * (kTokens / kCachePage));
-        keys[r] = values[r] = make_uint4(0, 0, 0, 0);
-        if (q >= 0) {
-          keys[r] = *reinterpret_cast<const uint4*>(key_codes + q * page_bytes);
-          values[r] = *reinterpret_cast<const uint4*>(value_codes + q * page_bytes);
-        }
-      }
-    };
-    auto widen = [](uint8_t* row, int lo, int hi, const uint4& x) {
-      *reinterpret_cast<uint4*>(row + lo) =
+    auto widen = [&](uint8_t* row, const uint4& x) {
+      *reinterpret_cast<uint4*>(row + chunk_lo) =
           make_uint4(e4m3x2_to_f16x2(x.x & 0xffffu), e4m3x2_to_f16x2(x.x >> 16),
                      e4m3x2_to_f16x2(x.y & 0xffffu), e4m3x2_to_f16x2(x.y >> 16));
-      *reinterpret_cast<uint4*>(row + hi) =
+      *reinterpret_cast<uint4*>(row + chunk_hi) =
           make_uint4(e4m3x2_to_f16x2(x.z & 0xffffu), e4m3x2_to_f16x2(x.z >> 16),
                      e4m3x2_to_f16x2(x.w & 0xffffu), e4m3x2_to_f16x2(x.w >> 16));
     };
-    auto put = [&](int j, const uint4 (&keys)[kRounds], const uint4 (&values)[kRounds]) {
-      const int stage = j % S::kStages;
-      const int step = step_begin + j;
-      const int entry = step * kStepPages;
+    for (int j = 0; j < steps; ++j) {
+      const int stage = j % S::kStages, slot = j % S::kStaged;
+      wait(&control.staged_full[slot], j / S::kStaged, kSiteStaged);
+      uint4 keys[kRounds], values[kRounds];
+      int token[kRounds];
+      const uint8_t* const codes = own_codes + slot * 2 * S::kCodeBytes;
+#pragma unroll
+      for (int r = 0; r < kRounds; ++r) {
+        keys[r] = *reinterpret_cast<const uint4*>(codes + r * kTokens * D);
+        values[r] = *reinterpret_cast<const uint4*>(codes + S::kCodeBytes + r * kTokens * D);
+        token[r] = control.pages[j % kInfoSteps][first_page + r * (kTokens / kCachePage)].token +
+                   first_token % kCachePage;
+      }
+      mbar_arrive(&control.staged_free[slot]);
       if (j >= S::kStages) wait(&control.tiles_free[stage], j / S::kStages - 1, kSiteFree);
       uint8_t* const tile = own_tile + stage * 2 * S::kTileBytes;
       bool any_nan = false;
 #pragma unroll
       for (int r = 0; r < kRounds; ++r) {
-        const int token = r * kTokens + first_token;
-        const int i = entry + r * (kTokens / kCachePage) + lane_page;
-        const int position = (i < v.front ? i : i - v.front + v.back) * kCachePage +
-                             first_token % kCachePage;
-        // values that no row sees, or that are NaN (the whole row then), must not meet the product
-        const bool unseen = position >= v.length;
-        const bool nan = (values[r].x & 0x7fu) == 0x7fu && !unseen;
+        // tokens that no row sees, or that are NaN (a whole row of codes then), become zeros; a
+        // page of nobody has negative tokens
+        const bool unseen = token[r] >= v.length || token[r] < 0;
+        const bool nan =
+            ((values[r].x & 0x7fu) == 0x7fu || (keys[r].x & 0x7fu) == 0x7fu) && !unseen;
         any_nan = any_nan || nan;
-        if (part == 0) control.row_nan[stage][token] = nan ? 1 : 0;
-        widen(tile + r * kTokens * 128, chunk_lo, chunk_hi, keys[r]);
-        widen(tile + S::kTileBytes + r * kTokens * 128, chunk_lo, chunk_hi,
-              nan || unseen ? make_uint4(0, 0, 0, 0) : values[r]);
+        if (part == 0) control.row_nan[stage][r * kTokens + first_token] = nan ? 1 : 0;
+        if (nan || unseen) keys[r] = values[r] = make_uint4(0, 0, 0, 0);
+        widen(tile + r * kTokens * 128, keys[r]);
+        widen(tile + S::kTileBytes + r * kTokens * 128, values[r]);
       }
       any_nan = __any_sync(0xffffffffu, any_nan);
       if (lane == 0) control.any_nan[stage][warp - kWidenWarp] = any_nan ? 1u : 0u;
-      if (warp == kWidenWarp) {
-        const int at = step % kSteps * kStepPages + (lane & (kStepPages - 1));
-        const int held = __shfl_sync(0xffffffffu, page, at);
-        const uint32_t scales = __shfl_sync(0xffffffffu, bytes, at);
-        if (lane < kStepPages) {
-          // a page of nobody gives weights of zero and asks for no masks
-          PageInfo info{0.0f, -INFINITY, 0.0f, -kStepTokens};
-          if (held >= 0) {
-            const int i = entry + lane;
-            const int e = scale_exponent(scales >> 8);
-            info = PageInfo{exp2_int(scale_exponent(scales & 0xffu)), static_cast<float>(e),
-                            exp2_int(-e), (i < v.front ? i : i - v.front + v.back) * kCachePage};
-          }
-          control.pages[stage][lane] = info;
-        }
-      }
       fence_proxy_async_smem();
       mbar_arrive(&control.tiles_full[stage]);
-      if ((step + 1) % kSteps == 0) {  // on to the next group of pages
-        ++group;
-        page = next_page;
-        bytes = next_bytes;
-        look_up(group + 1, next_page, next_bytes);
-      }
-    };
-    uint4 keys_a[kRounds], values_a[kRounds], keys_b[kRounds], values_b[kRounds];
-    if (steps > 0) load(0, keys_a, values_a);
-    for (int j = 0; j < steps; j += 2) {
-      if (j + 1 < steps) load(j + 1, keys_b, values_b);
-      put(j, keys_a, values_a);
-      if (j + 1 < steps) {
-        if (j + 2 < steps) load(j + 2, keys_a, values_a);
-        put(j + 1, keys_b, values_b);
-      }
     }
   }
 
