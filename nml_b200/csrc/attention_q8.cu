@@ -22,11 +22,13 @@
 #include <type_traits>
 
 #include "attention_q8.cuh"
+#include "sm100_primitives.cuh"
 
 namespace nml_sm100 {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr int kSiteRowCodes = 22;  // bit 8 + site of the status word: a wait for codes ran out
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -43,20 +45,38 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return r;
 }
 
+// Row r (of 8) of a score tile is token kTokenOrder(r) of its half page: neighbouring rows and every
+// second row fall on different halves of the shared-memory banks for 64-byte rows of codes.
+__device__ __forceinline__ int token_of_row(int r) { return r ^ ((r >> 1) & 1); }
+
+// Steps of kPages pages that a warp has in shared memory or on the way, and its bytes of them.
+template <int D>
+struct RowShape {
+  static constexpr int kPages = 128 / D;
+  static constexpr int kRing = 4;
+  static constexpr int kBlockBytes = kCachePage * D;
+  static constexpr int kStepBytes = 2 * kPages * kBlockBytes;  // keys, then values
+  static constexpr int kSharedBytes = kWarps * kRing * kStepBytes;
+};
+
 // NT: tiles of 8 query heads of one kv head that share the loaded codes.
-template <typename T, int D, int NT, int CP>
+template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32)
 row_kernel(const AttentionParams p) {
+  using S = RowShape<D>;
+  constexpr int CP = S::kPages;
   constexpr int KW = D / 16;   // 32-bit words of keys a lane holds for each of its two tokens
   constexpr int VW = D / 32;   // words of values a lane holds for each of its four tokens
   constexpr int kStride = D + 2;
+  extern __shared__ __align__(128) uint8_t ring_shared[];
+  __shared__ uint64_t full[kWarps][S::kRing];
+  __shared__ float merged[kWarps][8 * NT][kStride];
   const int split = blockIdx.x % p.splits;
   const int row = blockIdx.x / p.splits;
   const int kv_head = blockIdx.y / p.head_tiles;
   const int head_base = (blockIdx.y % p.head_tiles) * (8 * NT);  // within the group
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
-  __shared__ float merged[kWarps][8 * NT][kStride];
 
   const int sequence =
       p.offsets == nullptr ? row : sequence_of_row(p.offsets, p.cache.batch, row);
@@ -67,6 +87,57 @@ row_kernel(const AttentionParams p) {
   const int per_split = (v.pages + p.splits - 1) / p.splits;
   const int page_begin = split * per_split;
   const int page_end = min(v.pages, page_begin + per_split);
+  // this warp's steps: step k holds entries page_begin + (k * kWarps + warp) * CP ..
+  const int all_steps = max(0, (page_end - page_begin + CP - 1) / CP);
+  const int steps = (all_steps - warp + kWarps - 1) / kWarps;
+
+  if (lane == 0) {
+    for (int i = 0; i < S::kRing; ++i) mbar_init(&full[warp][i], 1);
+    mbar_fence_init();
+  }
+  __syncwarp();
+  uint8_t* const ring = ring_shared + warp * S::kRing * S::kStepBytes;
+
+  // Lane i holds what page i % CP of step kGroup * group + i / CP is: its block (-1: nothing
+  // there) and scale bytes; the next group's are under way.
+  constexpr int kGroup = 32 / CP;
+  int64_t block, next_block;
+  uint32_t key_byte, value_byte, next_key, next_value;
+  auto entry_of = [&](int step, int i) { return page_begin + (step * kWarps + warp) * CP + i; };
+  auto look_up = [&](int group, int64_t& at, uint32_t& key, uint32_t& value) {
+    at = -1;
+    key = value = 127;
+    const int i = entry_of(group * kGroup + lane / CP, lane % CP);
+    if (i < page_end) {
+      const int page = physical_page(p.cache, sequence, i < v.front ? i : i - v.front + v.back,
+                                     p.status);
+      if (page >= 0) {
+        at = static_cast<int64_t>(page) * p.cache.kv_heads + kv_head;
+        key = p.cache.scales[0][at];
+        value = p.cache.scales[1][at];
+      }
+    }
+  };
+  int group = 0;  // of the step worked on
+  look_up(0, block, key_byte, value_byte);
+  look_up(1, next_block, next_key, next_value);
+  // Brings step k's blocks into its slot, one bulk copy each, by the lanes that hold them.
+  auto fetch = [&](int k) {
+    const int64_t at = k / kGroup == group ? block : next_block;
+    const bool mine = lane / CP == k % kGroup && at >= 0;
+    const int slot = k % S::kRing;
+    const uint32_t count = __popc(__ballot_sync(0xffffffffu, mine));
+    if (lane == 0) mbar_arrive_expect_tx(&full[warp][slot], count * 2 * S::kBlockBytes);
+    __syncwarp();
+    if (mine) {
+      uint8_t* const to = ring + slot * S::kStepBytes + (lane % CP) * S::kBlockBytes;
+      bulk_load(to, p.cache.codes[0] + at * S::kBlockBytes, S::kBlockBytes, &full[warp][slot]);
+      bulk_load(to + CP * S::kBlockBytes, p.cache.codes[1] + at * S::kBlockBytes, S::kBlockBytes,
+                &full[warp][slot]);
+    }
+    __syncwarp();
+  };
+  for (int k = 0; k < min(steps, S::kRing); ++k) fetch(k);
 
   // Queries as B fragments: head g of every tile, the dimensions that this lane's key words hold
   // (word w of a token: dimensions 64 (w / 4) + 16 c + 4 (w % 4) .. + 3).
@@ -134,142 +205,89 @@ row_kernel(const AttentionParams p) {
     for (int i = 0; i < 2 * VW; ++i) out[n][i][0] = out[n][i][1] = out[n][i][2] = out[n][i][3] = 0;
   }
 
-  // Codes of a chunk: keys of tokens g and g + 8, values of tokens 2c, 2c+1, 2c+8, 2c+9.
-  uint32_t keys[CP][2][KW], values[CP][4][VW];
-  // lane i holds block index and scale bytes of page i of the chunk
-  int64_t block = -1;
-  uint32_t key_byte = 0, value_byte = 0;
-  auto look_up = [&](int index) {
-    block = -1;
-    key_byte = value_byte = 127;
-    if (lane < CP && index + lane < page_end) {
-      const int i = index + lane;
-      const int page = physical_page(p.cache, sequence, i < v.front ? i : i - v.front + v.back,
-                                     p.status);
-      if (page >= 0) {
-        block = static_cast<int64_t>(page) * p.cache.kv_heads + kv_head;
-        key_byte = p.cache.scales[0][block];
-        value_byte = p.cache.scales[1][block];
-      }
-    }
-  };
-  auto load_keys = [&]() {
-#pragma unroll
-    for (int i = 0; i < CP; ++i) {
-      const int64_t b = __shfl_sync(0xffffffffu, block, i);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int w = 0; w < KW; w += 4) {
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (b >= 0) {
-            x = *reinterpret_cast<const uint4*>(p.cache.codes[0] + b * (kCachePage * D) +
-                                                (g + 8 * h) * D + 64 * (w / 4) + 16 * c);
-          }
-          keys[i][h][w] = x.x; keys[i][h][w + 1] = x.y;
-          keys[i][h][w + 2] = x.z; keys[i][h][w + 3] = x.w;
-        }
-      }
-    }
-  };
-  auto load_values = [&]() {
-#pragma unroll
-    for (int i = 0; i < CP; ++i) {
-      const int64_t b = __shfl_sync(0xffffffffu, block, i);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const uint8_t* source = p.cache.codes[1] + b * (kCachePage * D) +
-                                (2 * c + (t & 1) + 8 * (t >> 1)) * D + (D / 8) * g;
-        if constexpr (VW == 2) {
-          uint2 x = make_uint2(0, 0);
-          if (b >= 0) x = *reinterpret_cast<const uint2*>(source);
-          values[i][t][0] = x.x; values[i][t][1] = x.y;
-        } else {
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (b >= 0) x = *reinterpret_cast<const uint4*>(source);
-          values[i][t][0] = x.x; values[i][t][1] = x.y;
-          values[i][t][2] = x.z; values[i][t][3] = x.w;
-        }
-      }
-    }
-  };
-
-  int index = page_begin + warp * CP;
-  if (index < page_end) {
-    look_up(index);
-    load_keys();
-    load_values();
-  }
-  for (; index < page_end; index += kWarps * CP) {
-    // visibility of this chunk's pages, then the next chunk's table entries
+  for (int k = 0; k < steps; ++k) {
+    const int slot = k % S::kRing;
     bool present[CP];
     float key_scale[CP], value_exponent[CP];
 #pragma unroll
     for (int i = 0; i < CP; ++i) {
-      present[i] = __shfl_sync(0xffffffffu, block, i) >= 0;
-      key_scale[i] = exp2_int(scale_exponent(__shfl_sync(0xffffffffu, key_byte, i)));
+      const int from = k % kGroup * CP + i;
+      present[i] = __shfl_sync(0xffffffffu, block, from) >= 0;
+      key_scale[i] = exp2_int(scale_exponent(__shfl_sync(0xffffffffu, key_byte, from)));
       value_exponent[i] =
-          static_cast<float>(scale_exponent(__shfl_sync(0xffffffffu, value_byte, i)));
+          static_cast<float>(scale_exponent(__shfl_sync(0xffffffffu, value_byte, from)));
     }
-    look_up(index + kWarps * CP);
+    if (!mbar_wait(&full[warp][slot], k / S::kRing & 1)) {
+      if (lane == 0) {
+        atomicOr(p.status, NML_SM100_STATUS_BARRIER_TIMEOUT | (0x100 << kSiteRowCodes));
+      }
+    }
+    __syncwarp();
+    const uint8_t* const codes = ring + slot * S::kStepBytes;
 
-    float s[NT][CP][4];  // tokens g (0, 1) and g + 8 (2, 3), heads 2c and 2c + 1
+    float s[NT][CP][4];  // tokens of rows g (0, 1) and g + 8 (2, 3), heads 2c and 2c + 1
 #pragma unroll
     for (int i = 0; i < CP; ++i) {
+      uint32_t keys[2][KW];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int w = 0; w < KW; w += 4) {
+          const uint4 x = *reinterpret_cast<const uint4*>(
+              codes + i * S::kBlockBytes + (token_of_row(g) + 8 * h) * D + 64 * (w / 4) + 16 * c);
+          keys[h][w] = x.x; keys[h][w + 1] = x.y;
+          keys[h][w + 2] = x.z; keys[h][w + 3] = x.w;
+        }
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n) s[n][i][0] = s[n][i][1] = s[n][i][2] = s[n][i][3] = 0.0f;
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
-        const uint32_t a0 = e4m3x2_to_f16x2(keys[i][0][w] & 0xffffu);
-        const uint32_t a2 = e4m3x2_to_f16x2(keys[i][0][w] >> 16);
-        const uint32_t a1 = e4m3x2_to_f16x2(keys[i][1][w] & 0xffffu);
-        const uint32_t a3 = e4m3x2_to_f16x2(keys[i][1][w] >> 16);
+        const uint32_t a0 = e4m3x2_to_f16x2(keys[0][w] & 0xffffu);
+        const uint32_t a2 = e4m3x2_to_f16x2(keys[0][w] >> 16);
+        const uint32_t a1 = e4m3x2_to_f16x2(keys[1][w] & 0xffffu);
+        const uint32_t a3 = e4m3x2_to_f16x2(keys[1][w] >> 16);
 #pragma unroll
         for (int n = 0; n < NT; ++n) mma_f16(s[n][i], a0, a1, a2, a3, q[n][w][0], q[n][w][1]);
       }
     }
-    if (index + kWarps * CP < page_end) load_keys();
 
     // scores into the exponent's domain; a page's tokens are masked only where some are unseen
-    float chunk_max[NT][2];
+    float step_max[NT][2];
+    bool whole[CP];
+    int first_token[CP];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) chunk_max[n][0] = chunk_max[n][1] = -INFINITY;
+    for (int n = 0; n < NT; ++n) step_max[n][0] = step_max[n][1] = -INFINITY;
+    auto seen = [&](int i, int t) {
+      return present[i] && t < v.length && (t >= v.start || t < p.first);
+    };
 #pragma unroll
     for (int i = 0; i < CP; ++i) {
-      const int logical = index + i < v.front ? index + i : index + i - v.front + v.back;
-      const int token = logical * kCachePage;
-      const bool whole = present[i] && token + kCachePage <= v.length &&
-                         (token >= v.start || token + kCachePage <= p.first);
+      const int entry = entry_of(k, i);
+      const int token = (entry < v.front ? entry : entry - v.front + v.back) * kCachePage;
+      first_token[i] = token;
+      whole[i] = present[i] && token + kCachePage <= v.length &&
+                 (token >= v.start || token + kCachePage <= p.first);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[n][i][j] *= factor[n][j & 1] * key_scale[i];
       }
-      if (!whole) {
-        auto seen = [&](int t) {
-          return present[i] && t < v.length && (t >= v.start || t < p.first);
-        };
-        const bool seen_g = seen(token + g), seen_h = seen(token + g + 8);
+      if (!whole[i]) {
+        const bool seen_g = seen(i, token + token_of_row(g));
+        const bool seen_h = seen(i, token + token_of_row(g) + 8);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           if (!seen_g) s[n][i][0] = s[n][i][1] = -INFINITY;
           if (!seen_h) s[n][i][2] = s[n][i][3] = -INFINITY;
         }
-        // whatever an unseen slot holds must not meet the product: 0 * NaN
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          if (!seen(token + 2 * c + (t & 1) + 8 * (t >> 1))) {
-#pragma unroll
-            for (int w = 0; w < VW; ++w) values[i][t][w] = 0;
-          }
-        }
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        chunk_max[n][0] = fmaxf(chunk_max[n][0],
-                                fmaxf(s[n][i][0], s[n][i][2]) + value_exponent[i]);
-        chunk_max[n][1] = fmaxf(chunk_max[n][1],
-                                fmaxf(s[n][i][1], s[n][i][3]) + value_exponent[i]);
+        step_max[n][0] = fmaxf(step_max[n][0],
+                               fmaxf(s[n][i][0], s[n][i][2]) + value_exponent[i]);
+        step_max[n][1] = fmaxf(step_max[n][1],
+                               fmaxf(s[n][i][1], s[n][i][3]) + value_exponent[i]);
       }
     }
     float base[NT][2];
@@ -277,7 +295,7 @@ row_kernel(const AttentionParams p) {
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float m = chunk_max[n][j];
+        float m = step_max[n][j];
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
@@ -309,12 +327,31 @@ row_kernel(const AttentionParams p) {
         weights[n][0] = transpose8x8(Elem<__half>::pack2(w0, w1));
         weights[n][1] = transpose8x8(Elem<__half>::pack2(w2, w3));
       }
+      uint32_t values[4][VW];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int token = token_of_row(2 * c + (t & 1)) + 8 * (t >> 1);
+        const uint8_t* const source = codes + (CP + i) * S::kBlockBytes + token * D + (D / 8) * g;
+        if constexpr (VW == 2) {
+          const uint2 x = *reinterpret_cast<const uint2*>(source);
+          values[t][0] = x.x; values[t][1] = x.y;
+        } else {
+          const uint4 x = *reinterpret_cast<const uint4*>(source);
+          values[t][0] = x.x; values[t][1] = x.y;
+          values[t][2] = x.z; values[t][3] = x.w;
+        }
+        // whatever an unseen slot holds must not meet the product: 0 * NaN
+        if (!whole[i] && !seen(i, first_token[i] + token)) {
+#pragma unroll
+          for (int w = 0; w < VW; ++w) values[t][w] = 0;
+        }
+      }
 #pragma unroll
       for (int w = 0; w < VW; ++w) {
-        const uint32_t lo01 = __byte_perm(values[i][0][w], values[i][1][w], 0x5140);
-        const uint32_t lo23 = __byte_perm(values[i][0][w], values[i][1][w], 0x7362);
-        const uint32_t hi01 = __byte_perm(values[i][2][w], values[i][3][w], 0x5140);
-        const uint32_t hi23 = __byte_perm(values[i][2][w], values[i][3][w], 0x7362);
+        const uint32_t lo01 = __byte_perm(values[0][w], values[1][w], 0x5140);
+        const uint32_t lo23 = __byte_perm(values[0][w], values[1][w], 0x7362);
+        const uint32_t hi01 = __byte_perm(values[2][w], values[3][w], 0x5140);
+        const uint32_t hi23 = __byte_perm(values[2][w], values[3][w], 0x7362);
         const uint32_t a[2][4] = {
             {e4m3x2_to_f16x2(lo01 & 0xffffu), e4m3x2_to_f16x2(lo01 >> 16),
              e4m3x2_to_f16x2(hi01 & 0xffffu), e4m3x2_to_f16x2(hi01 >> 16)},
@@ -330,7 +367,15 @@ row_kernel(const AttentionParams p) {
         }
       }
     }
-    if (index + kWarps * CP < page_end) load_values();
+    __syncwarp();  // every lane has its codes: the slot is free
+    if (k + S::kRing < steps) fetch(k + S::kRing);
+    if ((k + 1) % kGroup == 0) {
+      ++group;
+      block = next_block;
+      key_byte = next_key;
+      value_byte = next_value;
+      look_up(group + 1, next_block, next_key, next_value);
+    }
   }
 
   // ---- merge the warps ----
@@ -440,10 +485,15 @@ int32_t launch_attention(const AttentionParams& p, bool tiles, cudaStream_t stre
   if (tiles) {
     const int32_t code = launch_tiles<T, D>(p, stream, message, capacity);
     if (code != NML_SM100_OK) return code;
-  } else if (p.group <= 8) {
-    row_kernel<T, D, 1, 256 / D><<<grid, kWarps * 32, 0, stream>>>(p);
   } else {
-    row_kernel<T, D, 2, 128 / D><<<grid, kWarps * 32, 0, stream>>>(p);
+    auto kernel = p.group <= 8 ? row_kernel<T, D, 1> : row_kernel<T, D, 2>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             RowShape<D>::kSharedBytes) != cudaSuccess ||
+        cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                             cudaSharedmemCarveoutMaxShared) != cudaSuccess) {
+      return fail(NML_SM100_LAUNCH_FAILURE, "cannot configure shared memory", message, capacity);
+    }
+    kernel<<<grid, kWarps * 32, RowShape<D>::kSharedBytes, stream>>>(p);
   }
   if (p.splits > 1) {
     const int64_t heads = static_cast<int64_t>(p.tokens) * p.query_heads;
