@@ -49,11 +49,12 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 // second row fall on different halves of the shared-memory banks for 64-byte rows of codes.
 __device__ __forceinline__ int token_of_row(int r) { return r ^ ((r >> 1) & 1); }
 
-// Steps of kPages pages that a warp has in shared memory or on the way, and its bytes of them.
+// Steps of kPages pages that a warp has in shared memory or on the way, and its bytes of them
+// (figures: 64 sequences of 4097 tokens, 8 kv heads of 64).
 template <int D>
 struct RowShape {
   static constexpr int kPages = 128 / D;
-  static constexpr int kRing = 4;
+  static constexpr int kRing = 2;  // a deeper one costs resident CTAs: 53 us against 77 with four
   static constexpr int kBlockBytes = kCachePage * D;
   static constexpr int kStepBytes = 2 * kPages * kBlockBytes;  // keys, then values
   static constexpr int kSharedBytes = kWarps * kRing * kStepBytes;
@@ -71,10 +72,13 @@ row_kernel(const AttentionParams p) {
   extern __shared__ __align__(128) uint8_t ring_shared[];
   __shared__ uint64_t full[kWarps][S::kRing];
   __shared__ float merged[kWarps][8 * NT][kStride];
-  const int split = blockIdx.x % p.splits;
-  const int row = blockIdx.x / p.splits;
-  const int kv_head = blockIdx.y / p.head_tiles;
-  const int head_base = (blockIdx.y % p.head_tiles) * (8 * NT);  // within the group
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // the heads of a page lie side by side: CTAs next to each other read them at about one time
+  const int heads = p.cache.kv_heads * p.head_tiles;
+  const int kv_head = blockIdx.x % heads / p.head_tiles;
+  const int head_base = blockIdx.x % p.head_tiles * (8 * NT);  // within the group
+  const int split = blockIdx.x / heads % p.splits;
+  const int row = blockIdx.x / heads / p.splits;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
 
@@ -99,31 +103,33 @@ row_kernel(const AttentionParams p) {
   uint8_t* const ring = ring_shared + warp * S::kRing * S::kStepBytes;
 
   // Lane i holds what page i % CP of step kGroup * group + i / CP is: its block (-1: nothing
-  // there) and scale bytes; the next group's are under way.
+  // there), the factor of its scores and the exponent of its values; the next group's are under way.
   constexpr int kGroup = 32 / CP;
-  int64_t block, next_block;
-  uint32_t key_byte, value_byte, next_key, next_value;
+  struct Held {
+    int64_t block;
+    float key_scale, value_exponent;
+  };
   auto entry_of = [&](int step, int i) { return page_begin + (step * kWarps + warp) * CP + i; };
-  auto look_up = [&](int group, int64_t& at, uint32_t& key, uint32_t& value) {
-    at = -1;
-    key = value = 127;
+  auto look_up = [&](int group) {
+    Held held{-1, 1.0f, 0.0f};
     const int i = entry_of(group * kGroup + lane / CP, lane % CP);
     if (i < page_end) {
       const int page = physical_page(p.cache, sequence, i < v.front ? i : i - v.front + v.back,
                                      p.status);
       if (page >= 0) {
-        at = static_cast<int64_t>(page) * p.cache.kv_heads + kv_head;
-        key = p.cache.scales[0][at];
-        value = p.cache.scales[1][at];
+        held.block = static_cast<int64_t>(page) * p.cache.kv_heads + kv_head;
+        held.key_scale = exp2_int(scale_exponent(p.cache.scales[0][held.block]));
+        held.value_exponent =
+            static_cast<float>(scale_exponent(p.cache.scales[1][held.block]));
       }
     }
+    return held;
   };
   int group = 0;  // of the step worked on
-  look_up(0, block, key_byte, value_byte);
-  look_up(1, next_block, next_key, next_value);
+  Held held = look_up(0), next_held = look_up(1);
   // Brings step k's blocks into its slot, one bulk copy each, by the lanes that hold them.
   auto fetch = [&](int k) {
-    const int64_t at = k / kGroup == group ? block : next_block;
+    const int64_t at = k / kGroup == group ? held.block : next_held.block;
     const bool mine = lane / CP == k % kGroup && at >= 0;
     const int slot = k % S::kRing;
     const uint32_t count = __popc(__ballot_sync(0xffffffffu, mine));
@@ -205,17 +211,30 @@ row_kernel(const AttentionParams p) {
     for (int i = 0; i < 2 * VW; ++i) out[n][i][0] = out[n][i][1] = out[n][i][2] = out[n][i][3] = 0;
   }
 
+  // entries whose tokens are all seen
+  const int whole_begin =
+      v.start == 0 ? 0 : v.front + (v.start + kCachePage - 1) / kCachePage - v.back;
+  const int whole_end = min(page_end, v.front + v.length / kCachePage - v.back);
+  uint32_t there = __ballot_sync(0xffffffffu, held.block >= 0);
+  const int row_token = token_of_row(g);
+
   for (int k = 0; k < steps; ++k) {
     const int slot = k % S::kRing;
-    bool present[CP];
-    float key_scale[CP], value_exponent[CP];
+    const int entry = entry_of(k, 0);
+    const int at = k % kGroup * CP;  // lane of the step's first page
+    const uint32_t present = there >> at;
+    const bool whole = entry >= whole_begin && entry + CP <= whole_end &&
+                       (present & ((1u << CP) - 1u)) == (1u << CP) - 1u;
+    float score_factor[NT][CP][2], value_exponent[CP];
 #pragma unroll
     for (int i = 0; i < CP; ++i) {
-      const int from = k % kGroup * CP + i;
-      present[i] = __shfl_sync(0xffffffffu, block, from) >= 0;
-      key_scale[i] = exp2_int(scale_exponent(__shfl_sync(0xffffffffu, key_byte, from)));
-      value_exponent[i] =
-          static_cast<float>(scale_exponent(__shfl_sync(0xffffffffu, value_byte, from)));
+      const float key_scale = __shfl_sync(0xffffffffu, held.key_scale, at + i);
+      value_exponent[i] = __shfl_sync(0xffffffffu, held.value_exponent, at + i);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        score_factor[n][i][0] = factor[n][0] * key_scale;
+        score_factor[n][i][1] = factor[n][1] * key_scale;
+      }
     }
     if (!mbar_wait(&full[warp][slot], k / S::kRing & 1)) {
       if (lane == 0) {
@@ -234,7 +253,7 @@ row_kernel(const AttentionParams p) {
 #pragma unroll
         for (int w = 0; w < KW; w += 4) {
           const uint4 x = *reinterpret_cast<const uint4*>(
-              codes + i * S::kBlockBytes + (token_of_row(g) + 8 * h) * D + 64 * (w / 4) + 16 * c);
+              codes + i * S::kBlockBytes + (row_token + 8 * h) * D + 64 * (w / 4) + 16 * c);
           keys[h][w] = x.x; keys[h][w + 1] = x.y;
           keys[h][w + 2] = x.z; keys[h][w + 3] = x.w;
         }
@@ -251,81 +270,100 @@ row_kernel(const AttentionParams p) {
         for (int n = 0; n < NT; ++n) mma_f16(s[n][i], a0, a1, a2, a3, q[n][w][0], q[n][w][1]);
       }
     }
-
-    // scores into the exponent's domain; a page's tokens are masked only where some are unseen
-    float step_max[NT][2];
-    bool whole[CP];
-    int first_token[CP];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) step_max[n][0] = step_max[n][1] = -INFINITY;
-    auto seen = [&](int i, int t) {
-      return present[i] && t < v.length && (t >= v.start || t < p.first);
+    // tokens of page i that the row does not see
+    auto seen = [&](int i, int within) {
+      const int e = entry + i;
+      const int t = (e < v.front ? e : e - v.front + v.back) * kCachePage + within;
+      return (present >> i & 1u) != 0 && t < v.length && (t >= v.start || t < p.first);
     };
+    if (!whole) {
 #pragma unroll
-    for (int i = 0; i < CP; ++i) {
-      const int entry = entry_of(k, i);
-      const int token = (entry < v.front ? entry : entry - v.front + v.back) * kCachePage;
-      first_token[i] = token;
-      whole[i] = present[i] && token + kCachePage <= v.length &&
-                 (token >= v.start || token + kCachePage <= p.first);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[n][i][j] *= factor[n][j & 1] * key_scale[i];
-      }
-      if (!whole[i]) {
-        const bool seen_g = seen(i, token + token_of_row(g));
-        const bool seen_h = seen(i, token + token_of_row(g) + 8);
+      for (int i = 0; i < CP; ++i) {
+        const bool seen_g = seen(i, row_token), seen_h = seen(i, row_token + 8);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           if (!seen_g) s[n][i][0] = s[n][i][1] = -INFINITY;
           if (!seen_h) s[n][i][2] = s[n][i][3] = -INFINITY;
         }
       }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        step_max[n][0] = fmaxf(step_max[n][0],
-                               fmaxf(s[n][i][0], s[n][i][2]) + value_exponent[i]);
-        step_max[n][1] = fmaxf(step_max[n][1],
-                               fmaxf(s[n][i][1], s[n][i][3]) + value_exponent[i]);
-      }
     }
-    float base[NT][2];
+
+    // Weights against the maximum so far; only when their sum says that it does not serve (or when
+    // there is none) is the step's maximum formed and the step weighted again.
+    uint32_t weights[NT][CP][2];
+    float step_sum[NT][2];
+    bool missing = false;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
+      missing = missing || running_max[n][0] == -INFINITY || running_max[n][1] == -INFINITY;
+    }
+    bool with_maximum = __any_sync(0xffffffffu, missing);
+    while (true) {
+      if (with_maximum) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float m = step_max[n][j];
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-        m = fmaxf(m, running_max[n][j]);
-        // nothing seen yet: leave the (empty) state as it is
-        const float rescale = m == -INFINITY ? 1.0f : exp2_fast(running_max[n][j] - m);
-        base[n][j] = m == -INFINITY ? 0.0f : m;
-        running_max[n][j] = m;
-        running_sum[n][j] *= rescale;
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int i = 0; i < 2 * VW; ++i) {
-          out[n][i][j] *= rescale;
-          out[n][i][j + 2] *= rescale;
+          for (int j = 0; j < 2; ++j) {
+            float m = running_max[n][j];
+#pragma unroll
+            for (int i = 0; i < CP; ++i) {
+              m = fmaxf(m, fmaf(fmaxf(s[n][i][j], s[n][i][j + 2]), score_factor[n][i][j],
+                                value_exponent[i]));
+            }
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+            // nothing seen yet: leave the (empty) state as it is
+            const float rescale = m == -INFINITY ? 1.0f : exp2_fast(running_max[n][j] - m);
+            running_max[n][j] = m;
+            running_sum[n][j] *= rescale;
+#pragma unroll
+            for (int i = 0; i < 2 * VW; ++i) {
+              out[n][i][j] *= rescale;
+              out[n][i][j + 2] *= rescale;
+            }
+          }
         }
       }
+      float largest = 0.0f;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float base[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          base[j] = running_max[n][j] == -INFINITY ? 0.0f : running_max[n][j];
+          step_sum[n][j] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < CP; ++i) {
+          const float unscale = exp2_fast(-value_exponent[i]);
+          float w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            w[j] = exp2_fast(fmaf(s[n][i][j], score_factor[n][i][j & 1],
+                                  value_exponent[i] - base[j & 1]));
+          }
+          largest = fmaxf(largest, fmaxf(w[0] + w[2], w[1] + w[3]));
+          step_sum[n][0] = fmaf(w[0] + w[2], unscale, step_sum[n][0]);
+          step_sum[n][1] = fmaf(w[1] + w[3], unscale, step_sum[n][1]);
+          weights[n][i][0] = Elem<__half>::pack2(w[0], w[1]);
+          weights[n][i][1] = Elem<__half>::pack2(w[2], w[3]);
+        }
+      }
+      if (with_maximum || !__any_sync(0xffffffffu, largest > kLargestSum)) break;
+      with_maximum = true;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      running_sum[n][0] += step_sum[n][0];
+      running_sum[n][1] += step_sum[n][1];
     }
 #pragma unroll
     for (int i = 0; i < CP; ++i) {
-      const float unscale = exp2_fast(-value_exponent[i]);
-      uint32_t weights[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const float w0 = exp2_fast(s[n][i][0] + (value_exponent[i] - base[n][0]));
-        const float w1 = exp2_fast(s[n][i][1] + (value_exponent[i] - base[n][1]));
-        const float w2 = exp2_fast(s[n][i][2] + (value_exponent[i] - base[n][0]));
-        const float w3 = exp2_fast(s[n][i][3] + (value_exponent[i] - base[n][1]));
-        running_sum[n][0] = fmaf(w0 + w2, unscale, running_sum[n][0]);
-        running_sum[n][1] = fmaf(w1 + w3, unscale, running_sum[n][1]);
-        weights[n][0] = transpose8x8(Elem<__half>::pack2(w0, w1));
-        weights[n][1] = transpose8x8(Elem<__half>::pack2(w2, w3));
+        weights[n][i][0] = transpose8x8(weights[n][i][0]);
+        weights[n][i][1] = transpose8x8(weights[n][i][1]);
       }
       uint32_t values[4][VW];
 #pragma unroll
@@ -340,10 +378,15 @@ row_kernel(const AttentionParams p) {
           values[t][0] = x.x; values[t][1] = x.y;
           values[t][2] = x.z; values[t][3] = x.w;
         }
+      }
+      if (!whole) {
         // whatever an unseen slot holds must not meet the product: 0 * NaN
-        if (!whole[i] && !seen(i, first_token[i] + token)) {
 #pragma unroll
-          for (int w = 0; w < VW; ++w) values[t][w] = 0;
+        for (int t = 0; t < 4; ++t) {
+          if (!seen(i, token_of_row(2 * c + (t & 1)) + 8 * (t >> 1))) {
+#pragma unroll
+            for (int w = 0; w < VW; ++w) values[t][w] = 0;
+          }
         }
       }
 #pragma unroll
@@ -361,8 +404,8 @@ row_kernel(const AttentionParams p) {
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            mma_f16(out[n][2 * w + h], a[h][0], a[h][1], a[h][2], a[h][3], weights[n][0],
-                    weights[n][1]);
+            mma_f16(out[n][2 * w + h], a[h][0], a[h][1], a[h][2], a[h][3], weights[n][i][0],
+                    weights[n][i][1]);
           }
         }
       }
@@ -371,10 +414,9 @@ row_kernel(const AttentionParams p) {
     if (k + S::kRing < steps) fetch(k + S::kRing);
     if ((k + 1) % kGroup == 0) {
       ++group;
-      block = next_block;
-      key_byte = next_key;
-      value_byte = next_value;
-      look_up(group + 1, next_block, next_key, next_value);
+      held = next_held;
+      there = __ballot_sync(0xffffffffu, held.block >= 0);
+      next_held = look_up(group + 1);
     }
   }
 
@@ -439,24 +481,33 @@ row_kernel(const AttentionParams p) {
   }
 }
 
-// One warp per query head of a row: joins the splits, applies the sink, narrows.
+// One CTA per query head of a row: joins the splits, applies the sink, narrows.  Four warps take
+// the splits in turn.
 template <typename T, int D>
 __global__ void __launch_bounds__(128)
 join_kernel(const AttentionParams p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t query_head = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (query_head >= static_cast<int64_t>(p.tokens) * p.query_heads) return;
+  constexpr int kStride = D + 2;
+  __shared__ float shared_sum[4], shared_out[4][D];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t query_head = blockIdx.x;
   const int row = static_cast<int>(query_head / p.query_heads);
   if (p.offsets != nullptr && sequence_of_row(p.offsets, p.cache.batch, row) < 0) return;
-  const float* base = p.partial + query_head * p.splits * (D + 2);
+  // launched while the splits still run: everything above overlaps with them
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const float* base = p.partial + query_head * p.splits * kStride;
   float total_max = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) total_max = fmaxf(total_max, base[s * (D + 2) + D]);
+  for (int s = lane; s < p.splits; s += 32) total_max = fmaxf(total_max, base[s * kStride + D]);
+#pragma unroll
+  for (int offset = 16; offset > 0; offset >>= 1) {
+    total_max = fmaxf(total_max, __shfl_xor_sync(0xffffffffu, total_max, offset));
+  }
   float total_sum = 0.0f, acc[D / 32] = {};
-  for (int s = 0; s < p.splits; ++s) {
-    const float* part = base + s * (D + 2);
-    const float m = part[D];
-    const float weight = m == -INFINITY ? 0.0f : exp2f(m - total_max);
-    total_sum += part[D + 1] * weight;
+#pragma unroll 4
+  for (int s = warp; s < p.splits; s += 4) {
+    const float* part = base + s * kStride;
+    const float2 state = *reinterpret_cast<const float2*>(part + D);
+    const float weight = state.x == -INFINITY ? 0.0f : exp2f(state.x - total_max);
+    total_sum += state.y * weight;
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
       const float2 x = *reinterpret_cast<const float2*>(part + 64 * i + 2 * lane);
@@ -464,24 +515,35 @@ join_kernel(const AttentionParams p) {
       acc[2 * i + 1] = fmaf(x.y, weight, acc[2 * i + 1]);
     }
   }
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) {
+    shared_out[warp][64 * i + 2 * lane] = acc[2 * i];
+    shared_out[warp][64 * i + 2 * lane + 1] = acc[2 * i + 1];
+  }
+  if (lane == 0) shared_sum[warp] = total_sum;
+  __syncthreads();
+  if (threadIdx.x >= D / 2) return;
+  total_sum = shared_sum[0] + shared_sum[1] + shared_sum[2] + shared_sum[3];
   float denominator = total_sum;
   if (p.sinks != nullptr) {
     denominator += exp2f(p.sinks[query_head % p.query_heads] * kLog2e - total_max);
   }
   const float inverse = total_sum == 0.0f ? 0.0f : 1.0f / denominator;
-  T* out = static_cast<T*>(p.output) + query_head * D + 2 * lane;
+  float x[2] = {0.0f, 0.0f};
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) {
-    *reinterpret_cast<uint32_t*>(out + 64 * i) =
-        Elem<T>::pack2(acc[2 * i] * inverse, acc[2 * i + 1] * inverse);
+  for (int w = 0; w < 4; ++w) {
+    x[0] += shared_out[w][2 * threadIdx.x];
+    x[1] += shared_out[w][2 * threadIdx.x + 1];
   }
+  T* out = static_cast<T*>(p.output) + query_head * D + 2 * threadIdx.x;
+  *reinterpret_cast<uint32_t*>(out) = Elem<T>::pack2(x[0] * inverse, x[1] * inverse);
 }
 
 template <typename T, int D>
 int32_t launch_attention(const AttentionParams& p, bool tiles, cudaStream_t stream, char* message,
                          size_t capacity) {
-  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(p.tokens) * p.splits),
-                  static_cast<unsigned>(p.cache.kv_heads * p.head_tiles));
+  const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(p.tokens) * p.splits *
+                                              p.cache.kv_heads * p.head_tiles);
   if (tiles) {
     const int32_t code = launch_tiles<T, D>(p, stream, message, capacity);
     if (code != NML_SM100_OK) return code;
@@ -496,8 +558,19 @@ int32_t launch_attention(const AttentionParams& p, bool tiles, cudaStream_t stre
     kernel<<<grid, kWarps * 32, RowShape<D>::kSharedBytes, stream>>>(p);
   }
   if (p.splits > 1) {
-    const int64_t heads = static_cast<int64_t>(p.tokens) * p.query_heads;
-    join_kernel<T, D><<<static_cast<unsigned>((heads + 3) / 4), 128, 0, stream>>>(p);
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(p.tokens) * p.query_heads));
+    config.blockDim = dim3(128);
+    config.stream = stream;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    const cudaError_t status = cudaLaunchKernelEx(&config, join_kernel<T, D>, p);
+    if (status != cudaSuccess) {
+      return fail(NML_SM100_LAUNCH_FAILURE, cudaGetErrorString(status), message, capacity);
+    }
   }
   return launch_result(message, capacity);
 }
@@ -515,18 +588,32 @@ bool use_tiles(const NmlSm100PagedAttentionQ8& r) {
   return r.query_offsets != nullptr && r.tokens > r.cache.batch;
 }
 
-// Splits of the visible pages: until there are two CTAs for every SM, at least eight pages each.
+// Splits of the visible pages.  Every CTA of a launch should be resident at once, or the launch be
+// many waves of them: the splits with the least waves / splits win, each against what it costs
+// (partial results written, read and joined: about 6 per cent, and 2 for every split).  At least
+// eight pages each.  Measured on B200: 64 sequences of 4097 tokens and 8 kv heads (512 CTAs), 53 us
+// unsplit, 57 in two; 3 sequences of 60000 to 100000 tokens (24 CTAs, head_dim 128), 97 us in 24
+// splits, 135 in 12, 112 in 48.
 int64_t choose_splits(const NmlSm100PagedAttentionQ8& r) {
   if (r.splits > 0) return r.splits;
-  constexpr int64_t kWanted = 2 * 148;
-  const int64_t pairs =
-      r.cache.kv_heads * (use_tiles(r) ? query_tiles(r.tokens, r.cache.batch,
-                                                     r.query_heads / r.cache.kv_heads)
-                                       : r.tokens);
-  int64_t splits = (kWanted + pairs - 1) / pairs;
-  const int64_t most = most_pages(r) / 8;
-  if (splits > most) splits = most;
-  return splits < 1 ? 1 : splits > 64 ? 64 : splits;
+  const int64_t group = r.query_heads / r.cache.kv_heads;
+  const bool tiles = use_tiles(r);
+  const int64_t units = r.cache.kv_heads *
+                        (tiles ? query_tiles(r.tokens, r.cache.batch, group)
+                               : r.tokens * (group <= 8 ? 1 : (group + 15) / 16));
+  const int64_t slots = 148 * (tiles ? 2 : group <= 8 ? 4 : 2);
+  const int64_t most = most_pages(r) / 8 < 64 ? most_pages(r) / 8 : 64;
+  int64_t best = 1;
+  double least = static_cast<double>((units + slots - 1) / slots);
+  for (int64_t s = 2; s <= most; ++s) {
+    const double cost = static_cast<double>((units * s + slots - 1) / slots) / s *
+                        (1.06 + 0.02 * static_cast<double>(s));
+    if (cost < least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
 }
 
 bool valid_request(const NmlSm100PagedAttentionQ8& r) {
@@ -584,9 +671,7 @@ extern "C" int32_t nml_sm100_paged_attention_q8(const NmlSm100PagedAttentionQ8* 
                 error_message, error_message_capacity);
   }
   const int64_t splits = choose_splits(r);
-  if (r.tokens * splits > std::numeric_limits<int32_t>::max() ||
-      (r.tokens + r.cache.batch) * splits * r.cache.kv_heads >
-          std::numeric_limits<int32_t>::max()) {
+  if ((r.tokens + r.cache.batch) * splits * r.query_heads > std::numeric_limits<int32_t>::max()) {
     return fail(NML_SM100_INVALID_ARGUMENT, "invalid 8-bit paged attention request: too many rows",
                 error_message, error_message_capacity);
   }

@@ -7,6 +7,8 @@
 namespace nml_sm100 {
 
 constexpr float kLog2e = 1.4426950408889634f;
+// Sum of weights up to which the maximum so far still serves: F16 holds each of them.
+constexpr float kLargestSum = 16384.0f;
 
 struct AttentionParams {
   CacheQ8 cache;

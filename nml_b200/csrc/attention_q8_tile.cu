@@ -40,8 +40,6 @@ constexpr int kWidenThreads = 128;
 constexpr int kWidenWarp = 4, kMmaWarp = 8, kLoadWarp = 9;
 constexpr int kThreads = 384;  // the last two warps only give their registers
 constexpr int kLaunchRegisters = 80;  // of a thread: two CTAs fill an SM
-// Sum of a page's 16 weights up to which the maximum so far still serves: F16 holds each of them.
-constexpr float kLargestSum = 16384.0f;
 constexpr int kTmemColumns = 256;
 
 // Bits 8 + site of the status word say which wait ran out.
@@ -134,6 +132,7 @@ tile_kernel(const AttentionParams p) {
   __shared__ __align__(16) Control<D> control;
   volatile int* const abort_flag = &control.abort_flag;
 
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // through a shuffle: the compiler then knows the roles' branches and loops to be warp-uniform
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
