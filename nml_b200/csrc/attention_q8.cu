@@ -588,12 +588,12 @@ bool use_tiles(const NmlSm100PagedAttentionQ8& r) {
   return r.query_offsets != nullptr && r.tokens > r.cache.batch;
 }
 
-// Splits of the visible pages.  Every CTA of a launch should be resident at once, or the launch be
-// many waves of them: the splits with the least waves / splits win, each against what it costs
-// (partial results written, read and joined: about 6 per cent, and 2 for every split).  At least
-// eight pages each.  Measured on B200: 64 sequences of 4097 tokens and 8 kv heads (512 CTAs), 53 us
-// unsplit, 57 in two; 3 sequences of 60000 to 100000 tokens (24 CTAs, head_dim 128), 97 us in 24
-// splits, 135 in 12, 112 in 48.
+// Splits of the visible pages: the number with the least estimate of the launch's time, in units of
+// one page of head_dim 64 for a resident CTA (0.19 us): waves of CTAs, each as long as its pages and
+// a fixed 19 units, and 13 + 0.3 for every split to write and join partial results.  At least eight
+// pages each.  Measured on B200 (8 kv heads): 64 sequences of 4097 tokens, 52 us unsplit, 59 in two;
+// 128 of 1025, 32 unsplit, 43 in two; 16 of 4097, 18 in four, 32 unsplit; one of 131001, 33 in 64,
+// 901 unsplit; 3 of 60000 to 100000 with head_dim 128, 88 in 24, 129 in 12, 97 in 32.
 int64_t choose_splits(const NmlSm100PagedAttentionQ8& r) {
   if (r.splits > 0) return r.splits;
   const int64_t group = r.query_heads / r.cache.kv_heads;
@@ -602,13 +602,14 @@ int64_t choose_splits(const NmlSm100PagedAttentionQ8& r) {
                         (tiles ? query_tiles(r.tokens, r.cache.batch, group)
                                : r.tokens * (group <= 8 ? 1 : (group + 15) / 16));
   const int64_t slots = 148 * (tiles ? 2 : group <= 8 ? 4 : 2);
-  const int64_t most = most_pages(r) / 8 < 64 ? most_pages(r) / 8 : 64;
+  const int64_t pages = most_pages(r);
   int64_t best = 1;
-  double least = static_cast<double>((units + slots - 1) / slots);
-  for (int64_t s = 2; s <= most; ++s) {
-    const double cost = static_cast<double>((units * s + slots - 1) / slots) / s *
-                        (1.06 + 0.02 * static_cast<double>(s));
-    if (cost < least) {
+  double least = 0.0;
+  for (int64_t s = 1; s <= 64 && (s == 1 || pages / s >= 8); ++s) {
+    const double waves = static_cast<double>((units * s + slots - 1) / slots);
+    const double length = static_cast<double>(pages * r.cache.head_dim) / (64.0 * s);
+    const double cost = waves * (length + 19.0) + (s > 1 ? 13.0 + 0.3 * s : 0.0);
+    if (s == 1 || cost < least) {
       least = cost;
       best = s;
     }
