@@ -68,7 +68,7 @@ row_kernel(const AttentionParams p) {
   constexpr int CP = S::kPages;
   constexpr int KW = D / 16;   // 32-bit words of keys a lane holds for each of its two tokens
   constexpr int VW = D / 32;   // words of values a lane holds for each of its four tokens
-  constexpr int kStride = D + 2;
+  constexpr int kStride = kPartial<D>;
   extern __shared__ __align__(128) uint8_t ring_shared[];
   __shared__ uint64_t full[kWarps][S::kRing];
   __shared__ float merged[kWarps][8 * NT][kStride];
@@ -461,8 +461,7 @@ row_kernel(const AttentionParams p) {
     const int64_t query_head = static_cast<int64_t>(row) * p.query_heads + kv_head * p.group + head;
     if (p.splits > 1) {
       float* destination = p.partial + (query_head * p.splits + split) * kStride;
-      *reinterpret_cast<float2*>(destination + d0) = make_float2(acc[0], acc[1]);
-      *reinterpret_cast<float2*>(destination + d0 + 2) = make_float2(acc[2], acc[3]);
+      *reinterpret_cast<float4*>(destination + d0) = make_float4(acc[0], acc[1], acc[2], acc[3]);
       if (d0 == 0) {
         *reinterpret_cast<float2*>(destination + D) = make_float2(total_max, total_sum);
       }
@@ -481,17 +480,22 @@ row_kernel(const AttentionParams p) {
   }
 }
 
-// One CTA per query head of a row: joins the splits, applies the sink, narrows.  Four warps take
-// the splits in turn.
-template <typename T, int D>
+// Joins the splits of a row's query head, applies the sink, narrows: kJoinWarps warps for one, which
+// take its splits in turn (one where rows are many and splits few, four where it is the other way).
+template <typename T, int D, int kJoinWarps>
 __global__ void __launch_bounds__(128)
 join_kernel(const AttentionParams p) {
-  constexpr int kStride = D + 2;
+  constexpr int kStride = kPartial<D>;
+  constexpr int kHeads = 4 / kJoinWarps;  // of a CTA
   __shared__ float shared_sum[4], shared_out[4][D];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t query_head = blockIdx.x;
+  const int64_t query_head = static_cast<int64_t>(blockIdx.x) * kHeads + warp / kJoinWarps;
   const int row = static_cast<int>(query_head / p.query_heads);
-  if (p.offsets != nullptr && sequence_of_row(p.offsets, p.cache.batch, row) < 0) return;
+  // (a CTA of one head leaves as a whole)
+  if (row >= p.tokens ||
+      (p.offsets != nullptr && sequence_of_row(p.offsets, p.cache.batch, row) < 0)) {
+    return;
+  }
   // launched while the splits still run: everything above overlaps with them
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const float* base = p.partial + query_head * p.splits * kStride;
@@ -503,7 +507,7 @@ join_kernel(const AttentionParams p) {
   }
   float total_sum = 0.0f, acc[D / 32] = {};
 #pragma unroll 4
-  for (int s = warp; s < p.splits; s += 4) {
+  for (int s = warp % kJoinWarps; s < p.splits; s += kJoinWarps) {
     const float* part = base + s * kStride;
     const float2 state = *reinterpret_cast<const float2*>(part + D);
     const float weight = state.x == -INFINITY ? 0.0f : exp2f(state.x - total_max);
@@ -515,28 +519,36 @@ join_kernel(const AttentionParams p) {
       acc[2 * i + 1] = fmaf(x.y, weight, acc[2 * i + 1]);
     }
   }
+  if constexpr (kJoinWarps > 1) {
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) {
-    shared_out[warp][64 * i + 2 * lane] = acc[2 * i];
-    shared_out[warp][64 * i + 2 * lane + 1] = acc[2 * i + 1];
+    for (int i = 0; i < D / 64; ++i) {
+      *reinterpret_cast<float2*>(&shared_out[warp][64 * i + 2 * lane]) =
+          make_float2(acc[2 * i], acc[2 * i + 1]);
+    }
+    if (lane == 0) shared_sum[warp] = total_sum;
+    __syncthreads();
+    if (warp != 0) return;
+#pragma unroll
+    for (int w = 1; w < kJoinWarps; ++w) {
+      total_sum += shared_sum[w];
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) {
+        acc[2 * i] += shared_out[w][64 * i + 2 * lane];
+        acc[2 * i + 1] += shared_out[w][64 * i + 2 * lane + 1];
+      }
+    }
   }
-  if (lane == 0) shared_sum[warp] = total_sum;
-  __syncthreads();
-  if (threadIdx.x >= D / 2) return;
-  total_sum = shared_sum[0] + shared_sum[1] + shared_sum[2] + shared_sum[3];
   float denominator = total_sum;
   if (p.sinks != nullptr) {
     denominator += exp2f(p.sinks[query_head % p.query_heads] * kLog2e - total_max);
   }
   const float inverse = total_sum == 0.0f ? 0.0f : 1.0f / denominator;
-  float x[2] = {0.0f, 0.0f};
+  T* out = static_cast<T*>(p.output) + query_head * D + 2 * lane;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    x[0] += shared_out[w][2 * threadIdx.x];
-    x[1] += shared_out[w][2 * threadIdx.x + 1];
+  for (int i = 0; i < D / 64; ++i) {
+    *reinterpret_cast<uint32_t*>(out + 64 * i) =
+        Elem<T>::pack2(acc[2 * i] * inverse, acc[2 * i + 1] * inverse);
   }
-  T* out = static_cast<T*>(p.output) + query_head * D + 2 * threadIdx.x;
-  *reinterpret_cast<uint32_t*>(out) = Elem<T>::pack2(x[0] * inverse, x[1] * inverse);
 }
 
 template <typename T, int D>
@@ -562,12 +574,15 @@ int32_t launch_attention(const AttentionParams& p, bool tiles, cudaStream_t stre
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     early.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(p.tokens) * p.query_heads));
+    const int64_t query_heads = static_cast<int64_t>(p.tokens) * p.query_heads;
+    const bool many = query_heads > 4096;
+    config.gridDim = dim3(static_cast<unsigned>(many ? (query_heads + 3) / 4 : query_heads));
     config.blockDim = dim3(128);
     config.stream = stream;
     config.attrs = &early;
     config.numAttrs = 1;
-    const cudaError_t status = cudaLaunchKernelEx(&config, join_kernel<T, D>, p);
+    const cudaError_t status =
+        cudaLaunchKernelEx(&config, many ? join_kernel<T, D, 1> : join_kernel<T, D, 4>, p);
     if (status != cudaSuccess) {
       return fail(NML_SM100_LAUNCH_FAILURE, cudaGetErrorString(status), message, capacity);
     }
@@ -641,7 +656,7 @@ extern "C" size_t nml_sm100_paged_attention_q8_workspace_bytes(
   const int64_t splits = choose_splits(*request);
   if (splits <= 1) return 0;
   return static_cast<size_t>(request->tokens) * request->query_heads * splits *
-         (request->cache.head_dim + 2) * sizeof(float);
+         (request->cache.head_dim + 4) * sizeof(float);
 }
 
 extern "C" int32_t nml_sm100_paged_attention_q8(const NmlSm100PagedAttentionQ8* request,

@@ -15,13 +15,17 @@ struct AttentionParams {
   const void* query;
   const int32_t* offsets;  // [batch + 1] or null
   const float* sinks;
-  float* partial;          // [rows, query_heads, splits, D + 2]: out, maximum, sum
+  float* partial;          // [rows, query_heads, splits, D + 4]: out, maximum, sum, two unused
   void* output;
   int64_t query_token_stride, query_head_stride;
   int tokens, query_heads, group, head_tiles, splits, window, first;
   float scale_log2;
   int* status;
 };
+
+// Floats of a partial result: a multiple of 16 bytes.
+template <int D>
+constexpr int kPartial = D + 4;
 
 // 2^x to 2 units in the last place (CUDA's documented bound of ex2.approx); results below 2^-126
 // are zero.  exp2f() itself would spend two more instructions on those.

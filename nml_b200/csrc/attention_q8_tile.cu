@@ -86,7 +86,7 @@ struct Control {
   uint64_t query_full, drained;
   uint32_t tmem;
   int abort_flag;
-  int sequence, tile;
+  int sequence, first_row, rows, first_position;
   PageInfo pages[kInfoSteps][kStepPages];
   alignas(16) uint32_t any_nan[Shape<D>::kStages][4];  // read 16 bytes at a time
   uint8_t row_nan[Shape<D>::kStages][kStepTokens];
@@ -143,13 +143,16 @@ tile_kernel(const AttentionParams p) {
 
   // ---- which sequence, which of its tiles: the last tile (the longest walk) comes first ----
   if (warp == 0) {
-    int sequence = -1, tile = 0, passed = 0;
+    int sequence = -1, tile = 0, passed = 0, begin = 0, end = 0, given_end = 0, length = 0;
     for (int base = 0; base < p.cache.batch && sequence < 0; base += 32) {
       const int b = base + lane;
       int tiles = 0;
       if (b < p.cache.batch) {
-        const int rows = min(p.offsets[b + 1], p.tokens) - max(p.offsets[b], 0);
-        tiles = rows > 0 ? (rows + per_tile - 1) / per_tile : 0;
+        begin = max(p.offsets[b], 0);
+        given_end = p.offsets[b + 1];
+        length = p.cache.lengths[b];
+        end = min(given_end, p.tokens);
+        tiles = end > begin ? (end - begin + per_tile - 1) / per_tile : 0;
       }
       int upto = tiles;
 #pragma unroll
@@ -162,12 +165,23 @@ tile_kernel(const AttentionParams p) {
         const int at = __ffs(holds) - 1;
         sequence = base + at;
         tile = __shfl_sync(0xffffffffu, upto, at) - 1 - (item - passed);
+        begin = __shfl_sync(0xffffffffu, begin, at);
+        end = __shfl_sync(0xffffffffu, end, at);
+        given_end = __shfl_sync(0xffffffffu, given_end, at);
+        length = __shfl_sync(0xffffffffu, length, at);
       }
       passed += __shfl_sync(0xffffffffu, upto, 31);
     }
     if (lane == 0) {
+      const int most = p.cache.table_width * kCachePage;
+      if (sequence >= 0 && length > most) {
+        atomicOr(p.status, NML_SM100_STATUS_INDEX_RANGE);
+        length = most;
+      }
       control.sequence = sequence;
-      control.tile = tile;
+      control.first_row = begin + tile * per_tile;
+      control.rows = min(per_tile, end - control.first_row);
+      control.first_position = length - given_end + control.first_row;
     }
   }
   if (threadIdx.x == kMmaWarp * 32) {
@@ -193,12 +207,8 @@ tile_kernel(const AttentionParams p) {
   const int sequence = control.sequence;
   if (sequence < 0) return;  // more work items than tiles
 
-  const int begin = max(p.offsets[sequence], 0);
-  const int end = min(p.offsets[sequence + 1], p.tokens);
-  const int first_row = begin + control.tile * per_tile;
-  const int rows = min(per_tile, end - first_row);
-  const int first_position =
-      sequence_length(p.cache, sequence, p.status) - p.offsets[sequence + 1] + first_row;
+  const int first_row = control.first_row, rows = control.rows;
+  const int first_position = control.first_position;
   const Visible v = visible_pages(first_position + rows,
                                   p.window > 0 ? first_position + 1 - p.window : 0, p.first);
   const int all_steps = (v.pages + kStepPages - 1) / kStepPages;
@@ -210,10 +220,13 @@ tile_kernel(const AttentionParams p) {
     tmem_alloc(&control.tmem, kTmemColumns);
     tmem_relinquish_alloc_permit();
   }
-  tcgen05_fence_before_sync();
-  __syncthreads();
-  tcgen05_fence_after_sync();
-  const uint32_t tmem = __shfl_sync(0xffffffffu, control.tmem, 0);
+  uint32_t tmem = 0;
+  if (warp < kWidenWarp || warp == kMmaWarp) {  // the loads need not wait for tensor memory
+    tcgen05_fence_before_sync();
+    asm volatile("barrier.cta.sync.aligned 1, %0;" ::"n"(kSoftmaxThreads + 32) : "memory");
+    tcgen05_fence_after_sync();
+    tmem = __shfl_sync(0xffffffffu, control.tmem, 0);
+  }
 
   auto wait = [&](uint64_t* bar, int phase, int site) {
     mbar_wait_or_abort(bar, static_cast<uint32_t>(phase) & 1u, abort_flag, p.status, site);
@@ -300,8 +313,16 @@ tile_kernel(const AttentionParams p) {
     const int whole_end = max(whole_pages, 0) / kStepPages - step_begin;
 
     float running_max = -INFINITY, running_sum = 0.0f;
+    // a warp none of whose rows is anybody's hands over whatever its lanes hold: a row of the
+    // products depends on that row of weights only
+    const bool idle = warp * 32 >= rows * p.group;
     for (int j = 0; j < steps; ++j) {
       const int buffer = j % S::kBuffers, stage = j % S::kStages;
+      if (idle) {
+        wait(&control.scores_full[buffer], j / S::kBuffers, kSiteScores);
+        mbar_arrive(&control.weights_full[buffer]);
+        continue;
+      }
       const uint32_t columns = lanes + S::kScores + buffer * kStepTokens;
       const PageInfo* const pages = control.pages[j % kInfoSteps];
       wait(&control.tiles_full[stage], j / S::kStages, kSiteTiles);  // for the page data
@@ -449,7 +470,7 @@ tile_kernel(const AttentionParams p) {
       denominator += exp2f(p.sinks[head] * kLog2e - running_max);
     }
     const float inverse = running_sum == 0.0f ? 0.0f : 1.0f / denominator;
-    float* partial = p.partial + (query_head * p.splits + split) * (D + 2);
+    float* partial = p.partial + (query_head * p.splits + split) * kPartial<D>;
     T* out = static_cast<T*>(p.output) + query_head * D;
 #pragma unroll
     for (int c = 0; c < D; c += 16) {
@@ -463,8 +484,9 @@ tile_kernel(const AttentionParams p) {
       }
       if (live && p.splits > 1) {
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          *reinterpret_cast<uint2*>(partial + c + i) = make_uint2(x[i], x[i + 1]);
+        for (int i = 0; i < 16; i += 4) {
+          *reinterpret_cast<uint4*>(partial + c + i) =
+              make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
         }
       } else if (live) {
         uint32_t packed[8];
@@ -491,25 +513,35 @@ tile_kernel(const AttentionParams p) {
       // and scale bytes of entry i of a group of 32 pages, the next group's beside them.
       constexpr int kGroup = 32, kSteps = kGroup / kStepPages;
       constexpr uint32_t kBlockBytes = kCachePage * D;
-      auto look_up = [&](int group, int& page, uint32_t& key_byte, uint32_t& value_byte) {
+      constexpr int32_t kNoEntry = -2147483647 - 1;  // past the walk, unlike a bad table entry
+      auto table_entry = [&](int group) {
+        const int i = group * kGroup + lane;
+        return i >= step_begin * kStepPages && i < min(v.pages, (step_begin + steps) * kStepPages)
+                   ? p.cache.page_table[static_cast<int64_t>(sequence) * p.cache.table_width +
+                                        (i < v.front ? i : i - v.front + v.back)]
+                   : kNoEntry;
+      };
+      auto look_up = [&](int32_t entry, int& page, uint32_t& key_byte, uint32_t& value_byte) {
         page = -1;
         key_byte = value_byte = 0;
-        const int i = group * kGroup + lane;
-        if (i >= step_begin * kStepPages && i < min(v.pages, (step_begin + steps) * kStepPages)) {
-          page = physical_page(p.cache, sequence, i < v.front ? i : i - v.front + v.back,
-                               p.status);
-          if (page >= 0) {
-            const int64_t block = static_cast<int64_t>(page) * p.cache.kv_heads + kv_head;
-            key_byte = p.cache.scales[0][block];
-            value_byte = p.cache.scales[1][block];
-          }
+        if (entry == kNoEntry) return;
+        if (entry < 0 || entry >= p.cache.physical_pages) {
+          atomicOr(p.status, NML_SM100_STATUS_INDEX_RANGE);
+          return;
         }
+        page = entry;
+        const int64_t block = static_cast<int64_t>(page) * p.cache.kv_heads + kv_head;
+        key_byte = p.cache.scales[0][block];
+        value_byte = p.cache.scales[1][block];
       };
       int group = step_begin / kSteps;
       int page, next_page;
       uint32_t key_byte, value_byte, next_key, next_value;
-      look_up(group, page, key_byte, value_byte);
-      look_up(group + 1, next_page, next_key, next_value);
+      {
+        const int32_t entry = table_entry(group), next_entry = table_entry(group + 1);
+        look_up(entry, page, key_byte, value_byte);
+        look_up(next_entry, next_page, next_key, next_value);
+      }
       for (int j = 0; j < steps; ++j) {
         const int step = step_begin + j, slot = j % S::kStaged;
         if (j >= S::kStaged) wait(&control.staged_free[slot], j / S::kStaged - 1, kSiteFree);
@@ -549,7 +581,7 @@ tile_kernel(const AttentionParams p) {
           page = next_page;
           key_byte = next_key;
           value_byte = next_value;
-          look_up(group + 1, next_page, next_key, next_value);
+          look_up(table_entry(group + 1), next_page, next_key, next_value);
         }
       }
       // whatever has happened, no copy may land after the CTA is gone

@@ -110,7 +110,7 @@ def test_attention_scratch():
 
     refused(name, attention_request(dtype=9), "F16 and BF16 only")
     assert ask(splits=1) == 0
-    assert ask(splits=4) >= 2 * 16 * 4 * 66 * 4
+    assert ask(splits=4) >= 2 * 16 * 4 * 68 * 4
     refused(name, attention_request(splits=4), "workspace is too small")
     refused(name, attention_request(splits=4, workspace=FAKE, workspace_bytes=1000),
             "workspace is too small")
