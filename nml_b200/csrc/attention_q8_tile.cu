@@ -194,7 +194,7 @@ tile_kernel(const AttentionParams p) {
       mbar_init(&control.tiles_free[i], 1);
     }
     for (int i = 0; i < S::kBuffers; ++i) {
-      mbar_init(&control.scores_full[i], 1);
+      mbar_init(&control.scores_full[i], 2);
       mbar_init(&control.weights_full[i], kSoftmaxThreads);
       mbar_init(&control.product_done[i], 1);
     }
@@ -220,8 +220,24 @@ tile_kernel(const AttentionParams p) {
     tmem_alloc(&control.tmem, kTmemColumns);
     tmem_relinquish_alloc_permit();
   }
+  // A softmax thread's row; its queries (and sink) are on their way before tensor memory is waited
+  // for, which the loads of codes need not do at all.
+  const int token = threadIdx.x / p.group;
+  const int head = kv_head * p.group + threadIdx.x - token * p.group;
+  const bool live = warp < kWidenWarp && token < rows;
+  uint4 query[D / 8];
+  float sink = 0.0f;
   uint32_t tmem = 0;
-  if (warp < kWidenWarp || warp == kMmaWarp) {  // the loads need not wait for tensor memory
+  if (warp < kWidenWarp || warp == kMmaWarp) {
+    if (warp < kWidenWarp) {
+      const uint4* const source = reinterpret_cast<const uint4*>(
+          static_cast<const T*>(p.query) +
+          static_cast<int64_t>(first_row + token) * p.query_token_stride +
+          head * p.query_head_stride);
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) query[i] = live ? source[i] : make_uint4(0, 0, 0, 0);
+      if (p.sinks != nullptr && live) sink = p.sinks[head] * kLog2e;
+    }
     tcgen05_fence_before_sync();
     asm volatile("barrier.cta.sync.aligned 1, %0;" ::"n"(kSoftmaxThreads + 32) : "memory");
     tcgen05_fence_after_sync();
@@ -243,10 +259,6 @@ tile_kernel(const AttentionParams p) {
   if (warp < kWidenWarp) {
     // ------------------------------------------------------------------ softmax
     take_registers<S::kSoftmaxRegisters>();
-    const int row = threadIdx.x;
-    const int token = row / p.group;
-    const int head = kv_head * p.group + row - token * p.group;
-    const bool live = token < rows;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
     // rows of nobody walk like the last row, so that they do not ask for masks
     const int length = first_position + 1 + (live ? token : rows - 1);
@@ -256,19 +268,13 @@ tile_kernel(const AttentionParams p) {
     float factor = p.scale_log2;
     bool poisoned;  // something the row sees, or the row itself, is NaN: so is its result
     {
-      const T* source = static_cast<const T*>(p.query) +
-                        static_cast<int64_t>(first_row + token) * p.query_token_stride +
-                        head * p.query_head_stride;
       uint32_t largest = 0;  // magnitude bits in the upper half
-      if (live) {
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          const uint4 x = reinterpret_cast<const uint4*>(source)[i];
-          const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+      for (int i = 0; i < D / 8; ++i) {
+        const uint32_t words[4] = {query[i].x, query[i].y, query[i].z, query[i].w};
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            largest = max(largest, max((words[w] & 0x7fffu) << 16, words[w] & 0x7fff0000u));
-          }
+        for (int w = 0; w < 4; ++w) {
+          largest = max(largest, max((words[w] & 0x7fffu) << 16, words[w] & 0x7fff0000u));
         }
       }
       // a query with an infinity or a NaN gives NaN; its scores need not be formed
@@ -282,8 +288,7 @@ tile_kernel(const AttentionParams p) {
         uint32_t packed[8];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (live && !poisoned) x = reinterpret_cast<const uint4*>(source)[2 * i + h];
+          const uint4 x = poisoned ? make_uint4(0, 0, 0, 0) : query[2 * i + h];
           const uint32_t words[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
@@ -325,7 +330,8 @@ tile_kernel(const AttentionParams p) {
       }
       const uint32_t columns = lanes + S::kScores + buffer * kStepTokens;
       const PageInfo* const pages = control.pages[j % kInfoSteps];
-      wait(&control.tiles_full[stage], j / S::kStages, kSiteTiles);  // for the page data
+      wait(&control.scores_full[buffer], j / S::kBuffers, kSiteScores);
+      tcgen05_fence_after_sync();
       float page_factor[kStepPages], value_exponent[kStepPages], unscale[kStepPages];
 #pragma unroll
       for (int q = 0; q < kStepPages; ++q) {
@@ -336,8 +342,6 @@ tile_kernel(const AttentionParams p) {
       }
       const uint4 nan_words = *reinterpret_cast<const uint4*>(control.any_nan[stage]);
       const bool nans = (nan_words.x | nan_words.y | nan_words.z | nan_words.w) != 0;
-      wait(&control.scores_full[buffer], j / S::kBuffers, kSiteScores);
-      tcgen05_fence_after_sync();
 
       // Weights against the maximum so far; their sum tells whether it still serves.  Only when it
       // does not (or there is none yet) is the step's maximum formed and the step done again.
@@ -467,7 +471,7 @@ tile_kernel(const AttentionParams p) {
     if (poisoned) running_sum = __uint_as_float(0x7fc00000u);
     float denominator = running_sum;
     if (p.sinks != nullptr && live) {
-      denominator += exp2f(p.sinks[head] * kLog2e - running_max);
+      denominator += exp2f(sink - running_max);
     }
     const float inverse = running_sum == 0.0f ? 0.0f : 1.0f / denominator;
     float* partial = p.partial + (query_head * p.splits + split) * kPartial<D>;
@@ -606,6 +610,9 @@ tile_kernel(const AttentionParams p) {
                                 desc_hi | umma_desc_lo(address), score_idesc, k > 0 ? 1u : 0u);
         }
         umma_commit_elect(&control.scores_full[buffer]);
+        // a plain arrival too: it passes on what this warp saw at tiles_full, the page data
+        if (lane == 0) mbar_arrive(&control.scores_full[buffer]);
+        __syncwarp();
       };
       if (steps > 0) {
         wait(&control.query_full, 0, kSiteWeights);
