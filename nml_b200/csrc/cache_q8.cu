@@ -7,8 +7,6 @@
 namespace nml_sm100 {
 namespace {
 
-constexpr int kAppendThreads = 256;
-
 struct AppendParams {
   CacheQ8 cache;
   const void* source[2];  // key, value
@@ -34,52 +32,104 @@ __device__ __forceinline__ void load8(const T* address, float (&x)[8]) {
   }
 }
 
-// Elements [d0, d0 + 8) of a head's row after rotation by the angles of one position (`angles`:
-// cosines then sines, null for none).  Products and their sum are rounded one by one, so the
-// result does not depend on how the compiler contracts them.
-template <typename T, bool kInterleaved>
-__device__ __forceinline__ void rotated8(const T* row, int d0, const float* angles, int rotary_dim,
-                                         float (&x)[8]) {
-  load8(row + d0, x);
-  if (angles == nullptr || d0 >= rotary_dim) return;
-  const int half = rotary_dim >> 1;
-  if constexpr (kInterleaved) {
-    const float4 cos = *reinterpret_cast<const float4*>(angles + (d0 >> 1));
-    const float4 sin = *reinterpret_cast<const float4*>(angles + half + (d0 >> 1));
-    const float c[4] = {cos.x, cos.y, cos.z, cos.w}, s[4] = {sin.x, sin.y, sin.z, sin.w};
+template <typename T>
+__device__ __forceinline__ void store8(T* address, const float (&x)[8]) {
+  *reinterpret_cast<uint4*>(address) =
+      make_uint4(Elem<T>::pack2(x[0], x[1]), Elem<T>::pack2(x[2], x[3]),
+                 Elem<T>::pack2(x[4], x[5]), Elem<T>::pack2(x[6], x[7]));
+}
+
+// A head's row is cut into units of 16 elements that rotate among themselves: elements
+// [8u, 8u + 8) and their partners half the rotary width behind, or 16 neighbours (interleaved
+// pairs, and everything past the rotary width).  `a` and `b` are where its two halves lie.
+template <bool kInterleaved>
+__device__ __forceinline__ void unit_places(int unit, int rotary_dim, int& a, int& b) {
+  const bool apart = !kInterleaved && 16 * unit < rotary_dim;
+  a = apart ? 8 * unit : 16 * unit;
+  b = apart ? 8 * unit + (rotary_dim >> 1) : 16 * unit + 8;
+}
+
+// Angles of a unit at one position (`row` of the table: cosines, then sines); identity outside the
+// rotary width or without a table.
+struct Angles {
+  float cos[8], sin[8];
+  bool turn;
+};
+
+__device__ __forceinline__ Angles unit_angles(const float* row, int unit, int rotary_dim) {
+  Angles angles;
+  angles.turn = row != nullptr && 16 * unit < rotary_dim;
+  if (!angles.turn) return angles;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float a = x[2 * i], b = x[2 * i + 1];
-      x[2 * i] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i]));
-      x[2 * i + 1] = __fadd_rn(__fmul_rn(b, c[i]), __fmul_rn(a, s[i]));
-    }
-  } else {
-    const bool upper = d0 >= half;
-    const int index = upper ? d0 - half : d0;
-    float other[8];
-    load8(row + (upper ? d0 - half : d0 + half), other);
+  for (int j = 0; j < 2; ++j) {
+    const float4 c = *reinterpret_cast<const float4*>(row + 8 * unit + 4 * j);
+    const float4 s = *reinterpret_cast<const float4*>(row + (rotary_dim >> 1) + 8 * unit + 4 * j);
+    angles.cos[4 * j] = c.x; angles.cos[4 * j + 1] = c.y;
+    angles.cos[4 * j + 2] = c.z; angles.cos[4 * j + 3] = c.w;
+    angles.sin[4 * j] = s.x; angles.sin[4 * j + 1] = s.y;
+    angles.sin[4 * j + 2] = s.z; angles.sin[4 * j + 3] = s.w;
+  }
+  return angles;
+}
+
+// Products and their sum are rounded one by one, so that the result does not depend on how the
+// compiler contracts them.
+__device__ __forceinline__ void turn_pair(float& a, float& b, float cos, float sin) {
+  const float x = a, y = b;
+  a = __fsub_rn(__fmul_rn(x, cos), __fmul_rn(y, sin));
+  b = __fadd_rn(__fmul_rn(y, cos), __fmul_rn(x, sin));
+}
+
+template <bool kInterleaved>
+__device__ __forceinline__ void turn_unit(float (&a)[8], float (&b)[8], const Angles& angles) {
+  if (!angles.turn) return;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const float4 cos = *reinterpret_cast<const float4*>(angles + index + 4 * j);
-      const float4 sin = *reinterpret_cast<const float4*>(angles + half + index + 4 * j);
-      const float c[4] = {cos.x, cos.y, cos.z, cos.w}, s[4] = {sin.x, sin.y, sin.z, sin.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float own = __fmul_rn(x[4 * j + i], c[i]);
-        const float turn = __fmul_rn(other[4 * j + i], s[i]);
-        x[4 * j + i] = upper ? __fadd_rn(own, turn) : __fsub_rn(own, turn);
-      }
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (kInterleaved) {
+      float (&half)[8] = i < 4 ? a : b;
+      turn_pair(half[2 * (i & 3)], half[2 * (i & 3) + 1], angles.cos[i], angles.sin[i]);
+    } else {
+      turn_pair(a[i], b[i], angles.cos[i], angles.sin[i]);
     }
   }
 }
 
+__device__ __forceinline__ uint2 to_codes(const float (&x)[8], float inverse) {
+  uint32_t words[2];
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    words[w] = f32x2_to_e4m3x2(x[4 * w] * inverse, x[4 * w + 1] * inverse) |
+               f32x2_to_e4m3x2(x[4 * w + 2] * inverse, x[4 * w + 3] * inverse) << 16;
+  }
+  return make_uint2(words[0], words[1]);
+}
+
+// Codes at an exponent smaller by log2(shrink).
+__device__ __forceinline__ uint2 shrink_codes(uint2 old, float shrink) {
+  const uint32_t words[2] = {old.x, old.y};
+  float x[8];
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const uint32_t lo = e4m3x2_to_f16x2(words[w] & 0xffffu);
+    const uint32_t hi = e4m3x2_to_f16x2(words[w] >> 16);
+    x[4 * w] = Elem<__half>::from_bits(lo & 0xffffu);
+    x[4 * w + 1] = Elem<__half>::from_bits(lo >> 16);
+    x[4 * w + 2] = Elem<__half>::from_bits(hi & 0xffffu);
+    x[4 * w + 3] = Elem<__half>::from_bits(hi >> 16);
+  }
+  return to_codes(x, shrink);
+}
+
 // A CTA takes kChunk consecutive rows: first the sequence and position of each, then every block
 // whose first new row is among them (one warp for a block of one kv head's keys or values, all its
-// new rows at once, up to 16 of which may lie behind the chunk), then the chunk's query rows.
-template <typename T, int D, bool kInterleaved, int kChunk>
-__global__ void __launch_bounds__(kAppendThreads)
+// new rows at once, up to 15 of which may lie behind the chunk) and the chunk's query rows.  A lane
+// holds 16 elements of a row that rotate among themselves, so every element is read once, and the
+// angles of a query row's unit serve all its heads.
+template <typename T, int D, bool kInterleaved, int kChunk, int kThreads>
+__global__ void __launch_bounds__(kThreads)
 append_kernel(const AppendParams p) {
-  constexpr int kLanes = D / 8;            // lanes of a row, eight elements each
+  constexpr int kWarps = kThreads / 32;
+  constexpr int kLanes = D / 16;           // lanes of a row
   constexpr int kRows = 32 / kLanes;       // rows of one pass of a warp
   constexpr int kPasses = kCachePage / kRows;
   __shared__ int s_position[kChunk];       // -1: no row here, or nothing to write for it
@@ -94,10 +144,9 @@ append_kernel(const AppendParams p) {
       sequence = p.offsets == nullptr ? row : sequence_of_row(p.offsets, p.cache.batch, row);
       if (sequence >= 0) {
         const int begin = p.offsets == nullptr ? row : p.offsets[sequence];
-        const int end = p.offsets == nullptr ? row + 1 : min(p.offsets[sequence + 1], p.tokens);
-        const int given_end = p.offsets == nullptr ? end : p.offsets[sequence + 1];
-        const int length = p.cache.lengths[sequence];
-        position = length - given_end + row;
+        const int given_end = p.offsets == nullptr ? row + 1 : p.offsets[sequence + 1];
+        const int end = min(given_end, p.tokens);
+        position = p.cache.lengths[sequence] - given_end + row;
         const int limit = p.cache.table_width * kCachePage;
         const int usable = p.rotary == nullptr ? limit : min(limit, p.rotary_rows);
         if (position >= usable) {
@@ -115,55 +164,58 @@ append_kernel(const AppendParams p) {
     s_count[threadIdx.x] = count;
   }
   __syncthreads();
+  const int unit = lane % kLanes;
+  int place_a, place_b;
+  unit_places<kInterleaved>(unit, p.rotary_dim, place_a, place_b);
 
   // ---- keys and values ----
-  const int units = kChunk * p.cache.kv_heads * 2;
-  for (int unit = warp; unit < units; unit += kAppendThreads / 32) {
-    const int leader = unit / (p.cache.kv_heads * 2);
+  const int tasks = kChunk * p.cache.kv_heads * 2;
+  for (int task = warp; task < tasks; task += kWarps) {
+    const int leader = task / (p.cache.kv_heads * 2);
     const int count = s_count[leader];
     if (count == 0) continue;
-    const int head = (unit >> 1) % p.cache.kv_heads;
-    const int which = unit & 1;  // 0: keys, 1: values
+    const int head = (task >> 1) % p.cache.kv_heads;
+    const bool is_key = (task & 1) == 0;
     const int position = s_position[leader];
     const int lead = position % kCachePage;
     int page = 0;
     if (lane == 0) {
       page = physical_page(p.cache, s_sequence[leader], position / kCachePage, p.status);
     }
-    page = __shfl_sync(0xffffffffu, page, 0);
-    if (page < 0) continue;
-    const int64_t block = static_cast<int64_t>(page) * p.cache.kv_heads + head;
-    const bool is_key = which == 0;
-    uint8_t* codes = (is_key ? p.cache.codes[0] : p.cache.codes[1]) + block * (kCachePage * D);
-    uint8_t* scale = (is_key ? p.cache.scales[0] : p.cache.scales[1]) + block;
-    // tokens in front of the first new row are older ones of this sequence
-    const int before = lead > 0 ? scale_exponent(*scale) : kLowestExponent;
     const int64_t token_stride = is_key ? p.token_stride[0] : p.token_stride[1];
     const T* source = static_cast<const T*>(is_key ? p.source[0] : p.source[1]) +
                       static_cast<int64_t>(first_row + leader) * token_stride +
                       head * (is_key ? p.head_stride[0] : p.head_stride[1]);
-    const int d0 = 8 * (lane % kLanes);
-    float x[kPasses][8];
+    float a[kPasses][8], b[kPasses][8];
     uint32_t largest = 0;
     uint32_t bad = 0;  // bit i: the row of pass i holds an infinity or a NaN
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
       const int r = i * kRows + lane / kLanes;  // slot in the block
-      const bool live = r >= lead && r < lead + count;
-      if (live) {
+      if (r >= lead && r < lead + count) {
         const T* row = source + static_cast<int64_t>(r - lead) * token_stride;
-        const float* angles =
-            is_key && p.rotary != nullptr
-                ? p.rotary + static_cast<int64_t>(position - lead + r) * p.rotary_dim
-                : nullptr;
-        rotated8<T, kInterleaved>(row, d0, angles, p.rotary_dim, x[i]);
+        load8(row + place_a, a[i]);
+        load8(row + place_b, b[i]);
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[i][j] = 0.0f;
+        for (int j = 0; j < 8; ++j) a[i][j] = b[i][j] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int r = i * kRows + lane / kLanes;
+      if (is_key && p.rotary != nullptr && r >= lead && r < lead + count) {
+        turn_unit<kInterleaved>(
+            a[i], b[i],
+            unit_angles(p.rotary + static_cast<int64_t>(position - lead + r) * p.rotary_dim, unit,
+                        p.rotary_dim));
       }
       uint32_t m = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[i][j]) & 0x7fffffffu);
+      for (int j = 0; j < 8; ++j) {
+        m = max(m, max(__float_as_uint(a[i][j]) & 0x7fffffffu,
+                       __float_as_uint(b[i][j]) & 0x7fffffffu));
+      }
 #pragma unroll
       for (int offset = 1; offset < kLanes; offset <<= 1) {
         m = max(m, __shfl_xor_sync(0xffffffffu, m, offset));
@@ -175,26 +227,23 @@ append_kernel(const AppendParams p) {
       }
     }
     largest = __reduce_max_sync(0xffffffffu, largest);
+    page = __shfl_sync(0xffffffffu, page, 0);
+    if (page < 0) continue;
+    const int64_t block = static_cast<int64_t>(page) * p.cache.kv_heads + head;
+    uint8_t* codes = (is_key ? p.cache.codes[0] : p.cache.codes[1]) + block * (kCachePage * D);
+    uint8_t* scale = (is_key ? p.cache.scales[0] : p.cache.scales[1]) + block;
+    // tokens in front of the first new row are older ones of this sequence
+    const int before = lead > 0 ? scale_exponent(*scale) : kLowestExponent;
     const int exponent = max(block_exponent(largest), before);
     if (lead > 0 && exponent > before) {
       // older codes move to the grown exponent
       const float shrink = exp2_int(before - exponent);
       for (int r = lane / kLanes; r < lead; r += kRows) {
-        uint2* place = reinterpret_cast<uint2*>(codes + r * D + d0);
-        const uint2 old = *place;
-        const uint32_t words[2] = {old.x, old.y};
-        uint32_t again[2];
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const uint32_t lo = e4m3x2_to_f16x2(words[w] & 0xffffu);
-          const uint32_t hi = e4m3x2_to_f16x2(words[w] >> 16);
-          again[w] = f32x2_to_e4m3x2(Elem<__half>::from_bits(lo & 0xffffu) * shrink,
-                                     Elem<__half>::from_bits(lo >> 16) * shrink) |
-                     f32x2_to_e4m3x2(Elem<__half>::from_bits(hi & 0xffffu) * shrink,
-                                     Elem<__half>::from_bits(hi >> 16) * shrink)
-                         << 16;
-        }
-        *place = make_uint2(again[0], again[1]);
+        uint4* place = reinterpret_cast<uint4*>(codes + r * D + 16 * unit);
+        const uint4 old = *place;
+        const uint2 lo = shrink_codes(make_uint2(old.x, old.y), shrink);
+        const uint2 hi = shrink_codes(make_uint2(old.z, old.w), shrink);
+        *place = make_uint4(lo.x, lo.y, hi.x, hi.y);
       }
     }
     const float inverse = exp2_int(-exponent);
@@ -202,47 +251,47 @@ append_kernel(const AppendParams p) {
     for (int i = 0; i < kPasses; ++i) {
       const int r = i * kRows + lane / kLanes;
       if (r < lead || r >= lead + count) continue;
-      uint32_t words[2];
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        words[w] = f32x2_to_e4m3x2(x[i][4 * w] * inverse, x[i][4 * w + 1] * inverse) |
-                   f32x2_to_e4m3x2(x[i][4 * w + 2] * inverse, x[i][4 * w + 3] * inverse) << 16;
-      }
-      if (bad >> i & 1u) words[0] = words[1] = 0x7f7f7f7fu;
-      *reinterpret_cast<uint2*>(codes + r * D + d0) = make_uint2(words[0], words[1]);
+      const uint2 nan = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+      const bool is_bad = (bad >> i & 1u) != 0;
+      *reinterpret_cast<uint2*>(codes + r * D + place_a) = is_bad ? nan : to_codes(a[i], inverse);
+      *reinterpret_cast<uint2*>(codes + r * D + place_b) = is_bad ? nan : to_codes(b[i], inverse);
     }
     if (lane == 0) *scale = static_cast<uint8_t>(exponent + 127);
   }
 
   // ---- query rows ----
   if (p.query == nullptr) return;
-  const int per_row = p.query_heads * kLanes;
-  for (int item = threadIdx.x; item < kChunk * per_row; item += kAppendThreads) {
-    const int local = item / per_row;
-    const int rest = item - local * per_row;
-    const int head = rest / kLanes;
-    const int d0 = 8 * (rest % kLanes);
+  auto rotate_heads = [&](int local, int first_head, int head_step) {
     const int row = first_row + local;
-    if (row >= p.tokens || s_sequence[local] < 0) continue;  // outside every sequence: untouched
+    if (row >= p.tokens || s_sequence[local] < 0) return;  // outside every sequence: untouched
     const int position = s_position[local];
-    float x[8];
-    if (position >= 0) {
-      const T* source = static_cast<const T*>(p.query) +
-                        static_cast<int64_t>(row) * p.query_token_stride +
-                        head * p.query_head_stride;
-      const float* angles = p.rotary == nullptr
-                                ? nullptr
-                                : p.rotary + static_cast<int64_t>(position) * p.rotary_dim;
-      rotated8<T, kInterleaved>(source, d0, angles, p.rotary_dim, x);
-    } else {
+    const Angles angles = unit_angles(
+        p.rotary == nullptr || position < 0
+            ? nullptr
+            : p.rotary + static_cast<int64_t>(position) * p.rotary_dim,
+        unit, p.rotary_dim);
+    const T* source =
+        static_cast<const T*>(p.query) + static_cast<int64_t>(row) * p.query_token_stride;
+    T* out = static_cast<T*>(p.query_output) + static_cast<int64_t>(row) * p.output_token_stride;
+#pragma unroll 4
+    for (int head = first_head + lane / kLanes; head < p.query_heads; head += head_step) {
+      float a[8], b[8];
+      if (position >= 0) {
+        load8(source + head * p.query_head_stride + place_a, a);
+        load8(source + head * p.query_head_stride + place_b, b);
+        turn_unit<kInterleaved>(a, b, angles);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = 0.0f;
+        for (int j = 0; j < 8; ++j) a[j] = b[j] = 0.0f;
+      }
+      store8(out + head * p.output_head_stride + place_a, a);
+      store8(out + head * p.output_head_stride + place_b, b);
     }
-    T* out = static_cast<T*>(p.query_output) + static_cast<int64_t>(row) * p.output_token_stride +
-             head * p.output_head_stride + d0;
-    *reinterpret_cast<uint4*>(out) =
-        make_uint4(Elem<T>::pack2(x[0], x[1]), Elem<T>::pack2(x[2], x[3]),
-                   Elem<T>::pack2(x[4], x[5]), Elem<T>::pack2(x[6], x[7]));
+  };
+  if constexpr (kChunk == 1) {  // the warps share one row's heads
+    rotate_heads(0, (kWarps - 1 - warp) * kRows, kWarps * kRows);
+  } else {
+    for (int local = warp; local < kChunk; local += kWarps) rotate_heads(local, 0, kRows);
   }
 }
 
@@ -324,15 +373,15 @@ read_kernel(const ReadParams p) {
 
 template <typename T, int D, bool kInterleaved>
 void launch_append(const AppendParams& p, cudaStream_t stream) {
-  // Few rows: one row for a CTA, so that a decode batch spreads over the SMs.  Many: 16 rows, so
-  // that most CTAs own about one block of every head.
+  // Few rows: one row and many warps for a CTA, so that a decode batch spreads over the SMs.  Many:
+  // 16 rows, so that most CTAs own about one block of every head.
   if (p.offsets == nullptr || p.tokens < 1024) {
-    append_kernel<T, D, kInterleaved, 1>
-        <<<static_cast<unsigned>(p.tokens), kAppendThreads, 0, stream>>>(p);
+    append_kernel<T, D, kInterleaved, 1, 512>
+        <<<static_cast<unsigned>(p.tokens), 512, 0, stream>>>(p);
   } else {
-    append_kernel<T, D, kInterleaved, kCachePage>
+    append_kernel<T, D, kInterleaved, kCachePage, 256>
         <<<static_cast<unsigned>((static_cast<int64_t>(p.tokens) + kCachePage - 1) / kCachePage),
-           kAppendThreads, 0, stream>>>(p);
+           256, 0, stream>>>(p);
   }
 }
 
