@@ -126,7 +126,7 @@ __device__ __forceinline__ uint2 shrink_codes(uint2 old, float shrink) {
 // holds 16 elements of a row that rotate among themselves, so every element is read once, and the
 // angles of a query row's unit serve all its heads.
 template <typename T, int D, bool kInterleaved, int kChunk, int kThreads>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kChunk == 1 ? 1 : D == 64 ? 4 : 2)
 append_kernel(const AppendParams p) {
   constexpr int kWarps = kThreads / 32;
   constexpr int kLanes = D / 16;           // lanes of a row
@@ -135,7 +135,12 @@ append_kernel(const AppendParams p) {
   __shared__ int s_position[kChunk];       // -1: no row here, or nothing to write for it
   __shared__ int s_sequence[kChunk];
   __shared__ int s_count[kChunk];          // new rows of the block that starts at this row, else 0
-  const int first_row = blockIdx.x * kChunk;
+  // of two CTAs for a chunk of many rows one writes the cache, one rotates the queries
+  constexpr bool kApart = kChunk > 1;
+  const bool both = !kApart || p.query == nullptr;
+  const bool write_cache = both || (blockIdx.x & 1) != 0;
+  const bool rotate_query = p.query != nullptr && (both || (blockIdx.x & 1) == 0);
+  const int first_row = (both ? blockIdx.x : blockIdx.x >> 1) * kChunk;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x < kChunk) {
     const int row = first_row + threadIdx.x;
@@ -169,7 +174,7 @@ append_kernel(const AppendParams p) {
   unit_places<kInterleaved>(unit, p.rotary_dim, place_a, place_b);
 
   // ---- keys and values ----
-  const int tasks = kChunk * p.cache.kv_heads * 2;
+  const int tasks = write_cache ? kChunk * p.cache.kv_heads * 2 : 0;
   for (int task = warp; task < tasks; task += kWarps) {
     const int leader = task / (p.cache.kv_heads * 2);
     const int count = s_count[leader];
@@ -260,7 +265,7 @@ append_kernel(const AppendParams p) {
   }
 
   // ---- query rows ----
-  if (p.query == nullptr) return;
+  if (!rotate_query) return;
   auto rotate_heads = [&](int local, int first_head, int head_step) {
     const int row = first_row + local;
     if (row >= p.tokens || s_sequence[local] < 0) return;  // outside every sequence: untouched
@@ -379,9 +384,9 @@ void launch_append(const AppendParams& p, cudaStream_t stream) {
     append_kernel<T, D, kInterleaved, 1, 512>
         <<<static_cast<unsigned>(p.tokens), 512, 0, stream>>>(p);
   } else {
+    const int64_t chunks = (static_cast<int64_t>(p.tokens) + kCachePage - 1) / kCachePage;
     append_kernel<T, D, kInterleaved, kCachePage, 256>
-        <<<static_cast<unsigned>((static_cast<int64_t>(p.tokens) + kCachePage - 1) / kCachePage),
-           256, 0, stream>>>(p);
+        <<<static_cast<unsigned>(p.query == nullptr ? chunks : 2 * chunks), 256, 0, stream>>>(p);
   }
 }
 
