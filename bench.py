@@ -53,6 +53,9 @@ PROFILE_CASES = {
     "moe_t4096": "routed layer, 4096 tokens, 32 experts, top-4 (tcgen05 grouped kernels)",
     "embedding": "packed embedding gather, 8192 rows of the 201088 x 2880 table",
     "attention": "paged-attention decode, batch 64, 4096 prior tokens, 64 query / 8 kv heads",
+    "attention_q8": "the same decode batch over the 8-bit cache",
+    "prompt_q8": "a prompt of 1024 tokens behind 1024 over the 8-bit cache (tcgen05 kernel)",
+    "append_q8": "4096 tokens appended to the 8-bit cache, keys and 64 query heads rotated",
     "topk": "row-wise top-8 of 1024 x 201088 bf16 logits",
     "split_k": "2880->5760 linear at M=32; with --kernel-policy 2 the tcgen05 tile with K cut "
                "over a cluster of CTAs (by default the weight-streaming kernel takes it)",
@@ -931,6 +934,35 @@ def run_case(args) -> None:
         def fn():
             ops.paged_attention_decode(query, keys, values, table, lengths, sinks)
         nbytes = 2 * batch * (prior + 1) * kv_heads * dim * 2
+    elif args.case in ("attention_q8", "prompt_q8", "append_q8"):
+        heads, kv_heads, dim, page = 64, 8, 64, 16
+        batch, prior, new = {"attention_q8": (64, 4096, 1), "prompt_q8": (1, 1024, 1024),
+                             "append_q8": (1, 0, 4096)}[args.case]
+        total, tokens = prior + new, batch * new
+        width = -(-total // page)
+        cache = [torch.zeros(size, dtype=torch.uint8, device=device) for size in
+                 2 * [(batch * width, kv_heads, page, dim), (batch * width, kv_heads)]]
+        table = torch.randperm(batch * width, device=device, generator=generator) \
+            .view(batch, width).to(torch.int32).contiguous()
+        lengths = torch.full((batch,), total, dtype=torch.int32, device=device)
+        filled = torch.arange(batch + 1, dtype=torch.int32, device=device) * total
+        key, value = (normal((batch * total, kv_heads, dim), 1.0) for _ in range(2))
+        query, sinks = normal((tokens, heads, dim), 1.0), normal((heads,), 1.0, torch.float32)
+        ops.paged_append_q8(key, value, *cache, table, lengths, filled)
+        offsets = None if new == 1 else \
+            torch.arange(batch + 1, dtype=torch.int32, device=device) * new
+        if args.case == "append_q8":
+            rotary = ops.rotary_table(
+                150000.0 ** (-torch.arange(32, dtype=torch.float64, device=device) / 32), total)
+
+            def fn():
+                ops.paged_append_q8(key, value, *cache, table, lengths, offsets, query=query,
+                                    rotary=rotary)
+            nbytes = tokens * (4 * heads * dim + 6 * kv_heads * dim + 4 * dim)
+        else:
+            def fn():
+                ops.paged_attention_q8(query, *cache, table, lengths, offsets, sinks)
+            nbytes = 2 * batch * total * kv_heads * dim + 4 * tokens * heads * dim
     elif args.case == "split_k":
         weight = quantize.quantize_parameter("w", normal((5760, hidden)))
         x = normal((32, hidden), 1.0)

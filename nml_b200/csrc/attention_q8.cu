@@ -593,22 +593,27 @@ int32_t launch_attention(const AttentionParams& p, bool tiles, cudaStream_t stre
 // Pages that a row can see at most.
 int64_t most_pages(const NmlSm100PagedAttentionQ8& r) {
   if (r.sliding_window == 0) return r.cache.table_width;
+  // (a tile's rows see windows that start up to 127 tokens apart)
   const int64_t pages = (r.sliding_window + kCachePage - 1) / kCachePage + 1 +
                         (r.first_tokens + kCachePage - 1) / kCachePage;
   return pages < r.cache.table_width ? pages : r.cache.table_width;
 }
 
-// Runs of tokens go to the tile kernel, single tokens to the row kernel.
+// Runs of tokens go to the tile kernel, single tokens, and runs of fewer than three on average, to
+// the row kernel.  Measured (8 kv heads of 64, groups of 8): 16 sequences of two rows and 2000 tokens
+// 18 us by rows, 22 by tiles; of four rows 26 and 25; 64 of four rows 86 and 61.
 bool use_tiles(const NmlSm100PagedAttentionQ8& r) {
-  return r.query_offsets != nullptr && r.tokens > r.cache.batch;
+  return r.query_offsets != nullptr && r.tokens >= 3 * r.cache.batch;
 }
 
 // Splits of the visible pages: the number with the least estimate of the launch's time, in units of
-// one page of head_dim 64 for a resident CTA (0.19 us): waves of CTAs, each as long as its pages and
-// a fixed 19 units, and 13 + 0.3 for every split to write and join partial results.  At least eight
-// pages each.  Measured on B200 (8 kv heads): 64 sequences of 4097 tokens, 52 us unsplit, 59 in two;
-// 128 of 1025, 32 unsplit, 43 in two; 16 of 4097, 18 in four, 32 unsplit; one of 131001, 33 in 64,
-// 901 unsplit; 3 of 60000 to 100000 with head_dim 128, 88 in 24, 129 in 12, 97 in 32.
+// one page of head_dim 64 for a resident CTA of the row kernel (0.19 us): waves of CTAs, each as
+// long as its pages and a fixed part, and what partial results cost to write and join.  At least
+// eight pages each.  Measured on B200 (8 kv heads).  Rows: 64 sequences of 4097 tokens, 52 us
+// unsplit, 59 in two; 128 of 1025, 32 unsplit, 43 in two; 16 of 4097, 18 in four, 32 unsplit; one of
+// 131001, 33 in 64, 901 unsplit; 3 of 60000 to 100000 with head_dim 128, 88 in 24, 129 in 12.  Tiles
+// (an SM's two CTAs take as long as one after the other): one sequence of 64 rows and 4000 tokens,
+// 23 in four, 49 unsplit; 16 of 16 rows and 2000 tokens, 28 unsplit, 32 in two.
 int64_t choose_splits(const NmlSm100PagedAttentionQ8& r) {
   if (r.splits > 0) return r.splits;
   const int64_t group = r.query_heads / r.cache.kv_heads;
@@ -616,14 +621,18 @@ int64_t choose_splits(const NmlSm100PagedAttentionQ8& r) {
   const int64_t units = r.cache.kv_heads *
                         (tiles ? query_tiles(r.tokens, r.cache.batch, group)
                                : r.tokens * (group <= 8 ? 1 : (group + 15) / 16));
-  const int64_t slots = 148 * (tiles ? 2 : group <= 8 ? 4 : 2);
+  // (of tiles with few rows, whose exponentials do not fill an SM, two run side by side)
+  const bool few = r.tokens * group <= 64 * r.cache.batch;
+  const int64_t slots = 148 * (tiles ? (few ? 2 : 1) : group <= 8 ? 4 : 2);
+  const double fixed = tiles ? 25.0 : 19.0, page = tiles ? 0.85 : 1.0;
+  const double join = tiles ? 20.0 : 13.0, join_split = tiles ? 0.5 : 0.3;
   const int64_t pages = most_pages(r);
   int64_t best = 1;
   double least = 0.0;
   for (int64_t s = 1; s <= 64 && (s == 1 || pages / s >= 8); ++s) {
     const double waves = static_cast<double>((units * s + slots - 1) / slots);
-    const double length = static_cast<double>(pages * r.cache.head_dim) / (64.0 * s);
-    const double cost = waves * (length + 19.0) + (s > 1 ? 13.0 + 0.3 * s : 0.0);
+    const double length = page * static_cast<double>(pages * r.cache.head_dim) / (64.0 * s);
+    const double cost = waves * (length + fixed) + (s > 1 ? join + join_split * s : 0.0);
     if (s == 1 || cost < least) {
       least = cost;
       best = s;

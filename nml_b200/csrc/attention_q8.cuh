@@ -61,12 +61,12 @@ __device__ __forceinline__ Visible visible_pages(int length, int start, int firs
   return v;
 }
 
-// Rows of a query tile of the tile kernel and the number of its work items (an upper bound that
-// needs no device data).
+// Rows of a query tile of the tile kernel and the number of its work items: the most tiles that
+// the sequences' rows can need, which no device data is asked for.
 constexpr int kTileRows = 128;
 inline int64_t query_tiles(int64_t tokens, int64_t batch, int64_t group) {
   const int64_t per_tile = kTileRows / group;
-  return tokens / per_tile + (batch < tokens ? batch : tokens);
+  return (tokens + (per_tile - 1) * (batch < tokens ? batch : tokens)) / per_tile;
 }
 
 template <typename T, int D>

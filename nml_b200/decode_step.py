@@ -15,6 +15,11 @@ framework, as the reference leaves them on its graph: here they are plain torch 
 (RMSNorm, RoPE, cache write, router matmul, arg-max), stand-ins rather than tuned kernels.
 Every sequence owns a random set of physical KV pages.
 
+With ``cache="e4m3"`` the K/V cache is held in 8 bits with a scale for each page and kv head: RoPE
+and the cache write are one launch (``ops.paged_append_q8``) and attention reads half the bytes
+(``ops.paged_attention_q8``); ``DecodeModel.extend`` then also runs several new tokens of every
+sequence at once (prompts, chunks of them, drafted tokens).
+
 Several GPUs (one process each): sequences are sharded by batch (data-parallel attention, so
 the KV read divides too), experts are sharded with the peer-push schedule of
 ``expert_parallel.ExpertParallelMoE``, the vocabulary projection is column-sharded with a
@@ -107,8 +112,15 @@ class DecodeModel:
     """Random-init model state of one rank and the decode step over it."""
 
     def __init__(self, shape: GptOssShape, batch: int, prior_tokens: int, device, group=None,
-                 seed: int = 0, layers: int | None = None):
+                 seed: int = 0, layers: int | None = None, cache: str = "bf16", room: int = 1):
+        """``cache``: "bf16", or "e4m3" for the 8-bit cache; ``room``: tokens behind the prior ones
+        that the pages of every sequence have place for."""
+        if cache not in ("bf16", "e4m3"):
+            raise ValueError("the K/V cache is held in bf16 or e4m3")
+        if room < 1 or prior_tokens < 0:
+            raise ValueError("the cache needs place for at least one new token")
         self.shape = shape
+        self.quantized = cache == "e4m3"
         self.device = device
         self.group = group
         self.world = dist.get_world_size(group) if dist.is_initialized() else 1
@@ -119,7 +131,7 @@ class DecodeModel:
         self.batch = batch // self.world
         self.prior = prior_tokens
         self.layer_count = shape.layers if layers is None else layers
-        capacity = -(-(prior_tokens + 1) // shape.page_size) * shape.page_size
+        capacity = -(-(prior_tokens + room) // shape.page_size) * shape.page_size
         self.capacity = capacity
         # the same generator on every rank: replicated weights are identical, shards are cut
         # from identical full tensors
@@ -178,6 +190,10 @@ class DecodeModel:
             # paged KV cache of this rank's sequences, [pages, page_size, kv_heads, head_dim]
             # (crates/nml-ir/src/lib.rs:4717-4719); prior tokens hold random keys and values
             pages = self.batch * capacity // shape.page_size
+            if self.quantized:
+                layer["cache"] = self._empty_cache(pages)
+                self.layers.append(layer)
+                continue
             layer["key"] = normal((pages, shape.page_size, shape.key_value_heads, shape.head_dim),
                                   1.0)
             layer["value"] = normal((pages, shape.page_size, shape.key_value_heads,
@@ -188,15 +204,50 @@ class DecodeModel:
         self.page_table = order.view(self.batch, pages_per_sequence).to(torch.int32).contiguous()
         self.lengths = torch.full((self.batch,), prior_tokens + 1, dtype=torch.int32,
                                   device=device)
+        self.cached = [prior_tokens] * self.batch
         # where the new token's key and value go: (physical page, slot) of position `prior`
         self.write_page = self.page_table[:, prior_tokens // shape.page_size].long()
         self.write_slot = prior_tokens % shape.page_size
         frequencies, self.attention_factor = yarn_inverse_frequencies(shape, device)
+        if self.quantized:
+            self.rotary = ops.rotary_table(frequencies, capacity, self.attention_factor)
+            for layer in self.layers:
+                self._fill(layer, normal)
         angle = frequencies * float(prior_tokens)  # the step decodes position `prior_tokens`
         self.cos = (angle.cos() * self.attention_factor).to(dtype)
         self.sin = (angle.sin() * self.attention_factor).to(dtype)
         self.tokens = torch.randint(0, shape.vocabulary, (self.batch,), device=device,
                                     generator=g, dtype=torch.int32)
+
+    # ------------------------------------------------------------------ the 8-bit cache
+    def _empty_cache(self, pages: int) -> tuple:
+        """(key codes, key scales, value codes, value scales) of ``ops.paged_append_q8``."""
+        shape = self.shape
+        return tuple(
+            torch.zeros(size, dtype=torch.uint8, device=self.device)
+            for size in 2 * [(pages, shape.key_value_heads, shape.page_size, shape.head_dim),
+                             (pages, shape.key_value_heads)])
+
+    def _fill(self, layer, normal) -> None:
+        """Random prior tokens, written like any others (keys as if rotated already)."""
+        if self.prior == 0:
+            return
+        size = (self.batch * self.prior, self.shape.key_value_heads, self.shape.head_dim)
+        offsets = torch.arange(self.batch + 1, dtype=torch.int32, device=self.device) * self.prior
+        ops.paged_append_q8(normal(size, 1.0), normal(size, 1.0), *layer["cache"],
+                            self.page_table, torch.full_like(self.lengths, self.prior), offsets)
+
+    def _append_and_attend(self, layer, q, k, v, lengths, offsets) -> torch.Tensor:
+        shape, rows = self.shape, q.shape[0]
+        query = ops.paged_append_q8(
+            k.view(rows, shape.key_value_heads, shape.head_dim),
+            v.view(rows, shape.key_value_heads, shape.head_dim), *layer["cache"],
+            self.page_table, lengths, offsets,
+            query=q.view(rows, shape.query_heads, shape.head_dim), rotary=self.rotary)
+        out = ops.paged_attention_q8(
+            query, *layer["cache"], self.page_table, lengths, offsets, layer["sinks"],
+            sliding_window=shape.sliding_window if layer["sliding"] else None)
+        return out.view(rows, shape.query_width)
 
     # ------------------------------------------------------------------ pieces
     def _rope(self, x: torch.Tensor) -> torch.Tensor:
@@ -220,23 +271,67 @@ class DecodeModel:
         return ops.routed_clamped_swiglu(hidden, logits, gate_up, gate_bias, down, down_bias,
                                          self.shape.experts_per_token)
 
-    # ------------------------------------------------------------------ the step
-    def step(self) -> torch.Tensor:
-        """Decodes one token for every sequence of this rank; returns the next token ids."""
+    def _write_and_attend(self, layer, q, k, v) -> torch.Tensor:
+        """The 16-bit cache: one new token of every sequence."""
+        shape = self.shape
+        q = self._rope(q.view(self.batch, shape.query_heads, shape.head_dim))
+        k = self._rope(k.view(self.batch, shape.key_value_heads, shape.head_dim))
+        layer["key"][self.write_page, self.write_slot] = k
+        layer["value"][self.write_page, self.write_slot] = v.view(
+            self.batch, shape.key_value_heads, shape.head_dim)
+        return self._attention(layer, q)
+
+    def _run_layers(self, hidden: torch.Tensor, attend) -> torch.Tensor:
         shape, eps = self.shape, self.shape.rms_norm_eps
-        hidden = ops.token_embedding(self.table, self.tokens)
         for layer in self.layers:
             x = F.rms_norm(hidden, (shape.hidden,), layer["input_norm"], eps)
             q, k, v = ops.linear_qkv(x, layer["q"], layer["q_bias"], layer["k"], layer["k_bias"],
                                      layer["v"], layer["v_bias"])
-            q = self._rope(q.view(self.batch, shape.query_heads, shape.head_dim))
-            k = self._rope(k.view(self.batch, shape.key_value_heads, shape.head_dim))
-            layer["key"][self.write_page, self.write_slot] = k
-            layer["value"][self.write_page, self.write_slot] = v.view(
-                self.batch, shape.key_value_heads, shape.head_dim)
-            attention = self._attention(layer, q)
-            hidden = ops.linear(attention, layer["o"], layer["o_bias"], residual=hidden)
+            hidden = ops.linear(attend(layer, q, k, v), layer["o"], layer["o_bias"],
+                                residual=hidden)
             x = F.rms_norm(hidden, (shape.hidden,), layer["post_norm"], eps)
             hidden = hidden + self._moe(layer, x)
-        x = F.rms_norm(hidden, (shape.hidden,), self.final_norm, eps)
+        return hidden
+
+    def _pick(self, hidden: torch.Tensor) -> torch.Tensor:
+        x = F.rms_norm(hidden, (self.shape.hidden,), self.final_norm, self.shape.rms_norm_eps)
         return self.head.argmax(x)
+
+    # ------------------------------------------------------------------ the step
+    def step(self) -> torch.Tensor:
+        """Decodes one token for every sequence of this rank, at the position behind the prior
+        tokens; returns the next token ids."""
+        hidden = ops.token_embedding(self.table, self.tokens)
+        if self.quantized:
+            def attend(layer, q, k, v):
+                return self._append_and_attend(layer, q, k, v, self.lengths, None)
+        else:
+            attend = self._write_and_attend
+        return self._pick(self._run_layers(hidden, attend))
+
+    def extend(self, tokens: torch.Tensor, counts: list[int] | None = None) -> torch.Tensor:
+        """Runs the next ``counts[b]`` tokens of every sequence (one each without ``counts``; a
+        sequence may get none) through the model and keeps them in the 8-bit cache.  ``tokens``
+        holds them one sequence after the other; returns the next token id behind each of them."""
+        if not self.quantized or self.world > 1:
+            raise ValueError("extend runs over the e4m3 cache of one rank")
+        counts = [1] * self.batch if counts is None else list(counts)
+        if len(counts) != self.batch or min(counts) < 0 or sum(counts) != tokens.numel() or \
+                sum(counts) == 0:
+            raise ValueError("extend expects a count of new tokens for every sequence")
+        cached = [have + new for have, new in zip(self.cached, counts)]
+        if max(cached) > self.capacity:
+            raise ValueError(f"the cache has place for {self.capacity} tokens of a sequence")
+        offsets = None
+        if counts != [1] * self.batch:
+            offsets = torch.zeros(self.batch + 1, dtype=torch.int32)
+            offsets[1:] = torch.tensor(counts).cumsum(0)
+            offsets = offsets.to(self.device)
+        lengths = torch.tensor(cached, dtype=torch.int32).to(self.device)
+
+        def attend(layer, q, k, v):
+            return self._append_and_attend(layer, q, k, v, lengths, offsets)
+
+        hidden = self._run_layers(ops.token_embedding(self.table, tokens), attend)
+        self.cached = cached
+        return self._pick(hidden)

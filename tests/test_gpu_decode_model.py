@@ -1,0 +1,91 @@
+"""The decode model over the 8-bit cache: prompts in chunks, then single tokens, through the model's
+own entry points; what its first layer caches is checked against the projection of the embeddings."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+import cache_q8_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def small_shape():
+    from nml_b200.decode_step import GptOssShape
+    return GptOssShape(layers=2, hidden=256, intermediate=128, query_heads=16, key_value_heads=2,
+                       experts=4, experts_per_token=2, vocabulary=1000)
+
+
+def test_prompts_then_tokens():
+    from nml_b200 import _abi, ops
+    from nml_b200.decode_step import DecodeModel
+    shape = small_shape()
+    model = DecodeModel(shape, 3, 0, torch.device("cuda"), cache="e4m3", room=80)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    given = [[], [], []]
+    for counts in ([40, 1, 17], [9, 20, 0], None, None):
+        new = [1, 1, 1] if counts is None else counts
+        tokens = torch.randint(0, shape.vocabulary, (sum(new),), device="cuda", generator=gen,
+                               dtype=torch.int32)
+        out = model.extend(tokens, counts)
+        assert out.shape == (sum(new),) and int(out.min()) >= 0
+        assert int(out.max()) < shape.vocabulary
+        for b, part in enumerate(tokens.split(new)):
+            given[b] += part.tolist()
+    torch.cuda.synchronize()
+    assert _abi.device_status(0x1) == 0
+    assert model.cached == [51, 23, 19]
+    # layer 0's keys and values follow from the embeddings alone
+    layer = model.layers[0]
+    key, key_scales, value, value_scales = (x.cpu() for x in layer["cache"])
+    table = model.page_table.cpu()
+    for b, ids in enumerate(given):
+        hidden = ops.token_embedding(model.table, torch.tensor(ids, dtype=torch.int32).cuda())
+        x = F.rms_norm(hidden, (shape.hidden,), layer["input_norm"], shape.rms_norm_eps)
+        heads = (len(ids), shape.key_value_heads, shape.head_dim)
+        # the projections of a row do not depend on its batch beyond the order of f32 sums: one
+        # step of the result's type, 2^-7 of it or of the largest products' sum, is allowed beside
+        # half a code step (2^-4; two roundings where a block has grown)
+        for name, codes, scales in (("k", key, key_scales), ("v", value, value_scales)):
+            rows = ops.linear(x, layer[name], layer[name + "_bias"]).view(heads).cpu().double()
+            slack = rows.abs().amax(-1, keepdim=True) * 2.0 ** -7
+            if name == "k":
+                rows = ref.rotate(rows, model.rotary[: len(ids)].cpu(), "half")
+                slack = slack * 2 * model.attention_factor
+            held, _, exponent = ref.gather(codes, scales, table[b], len(ids))
+            limit = rows.abs() * 2.0 ** -4 * 1.07 + slack + \
+                2 * 2.0 ** -10 * torch.exp2(exponent)[..., None]
+            assert ((held - rows).abs() <= limit).all()
+
+
+def test_a_step_over_either_cache():
+    """The benchmark's step: both caches hold random prior tokens, the step runs and can be
+    captured into a graph that gives the same tokens again."""
+    from nml_b200 import _abi
+    from nml_b200.decode_step import DecodeModel
+    for cache in ("bf16", "e4m3"):
+        model = DecodeModel(small_shape(), 4, 70, torch.device("cuda"), cache=cache)
+        eager = model.step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = model.step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert _abi.device_status(0x1) == 0
+        assert torch.equal(out, eager)
+
+
+def test_extend_refusals():
+    from nml_b200.decode_step import DecodeModel
+    device = torch.device("cuda")
+    with pytest.raises(ValueError):
+        DecodeModel(small_shape(), 2, 0, device, cache="fp4")
+    with pytest.raises(ValueError):
+        DecodeModel(small_shape(), 2, 0, device, cache="e4m3", room=0)
+    tokens = torch.zeros(40, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError):
+        DecodeModel(small_shape(), 2, 0, device).extend(tokens[:2])
+    model = DecodeModel(small_shape(), 2, 0, device, cache="e4m3", room=20)
+    for count, counts in ((2, [1]), (2, [3, -1]), (3, [1, 1]), (0, [0, 0]), (40, [33, 7])):
+        with pytest.raises(ValueError):
+            model.extend(tokens[:count], counts)
+    assert model.cached == [0, 0]
