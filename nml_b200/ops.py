@@ -560,6 +560,12 @@ def rotary_table(frequencies: torch.Tensor, positions: int,
     return (torch.cat((angles.cos(), angles.sin()), dim=1) * attention_factor).float()
 
 
+def _stream_on(device: torch.device) -> int:
+    """``_stream`` without building a stream object: these calls are a few microseconds long."""
+    handle = torch._C._cuda_getCurrentRawStream(device.index)
+    return handle if handle != 0 else 0x1
+
+
 def _call_on(device: torch.device, name: str, request) -> None:
     """The library launches on the current device; make that the tensors' own."""
     if device.index == torch.cuda.current_device():
@@ -582,9 +588,9 @@ def _cache_q8(key_cache, key_scales, value_cache, value_scales, page_table, sequ
             sequence_lengths is not None and (sequence_lengths.dtype != torch.int32 or
                                               sequence_lengths.shape != (batch,))):
         raise ValueError("page table must be I32 [batch, pages], sequence lengths I32 [batch]")
-    for tensor in (key_cache, key_scales, value_cache, value_scales):
-        if tensor.dtype != torch.uint8:
-            raise ValueError("8-bit caches and their scales must use U8 buffers")
+    if not (key_cache.dtype is key_scales.dtype is value_cache.dtype is value_scales.dtype is
+            torch.uint8):
+        raise ValueError("8-bit caches and their scales must use U8 buffers")
     for tensor in (key_cache, key_scales, value_cache, value_scales, page_table,
                    sequence_lengths):
         if tensor is None:
@@ -676,7 +682,7 @@ def paged_append_q8(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Ten
     rotary_rows, rotary_dim = (0, 0) if rotary is None else rotary.shape
     request = _abi.PagedAppendQ8(
         0, cache, key.data_ptr(), value.data_ptr(), _ptr(query), _ptr(rotated),
-        _ptr(token_offsets), _ptr(rotary), _stream(key), tokens, heads, *key_strides,
+        _ptr(token_offsets), _ptr(rotary), _stream_on(device), tokens, heads, *key_strides,
         *value_strides, *query_strides, heads * dim, dim, rotary_rows, rotary_dim,
         1 if rotary_layout == "interleaved" else 0, dtype)
     _call_on(device, "nml_sm100_paged_append_q8", request)
@@ -712,7 +718,7 @@ def paged_read_q8(key_cache: torch.Tensor, key_scales: torch.Tensor, value_cache
     if tokens == 0:
         return out
     request = _abi.PagedReadQ8(0, cache, token_offsets.data_ptr(), out[0].data_ptr(),
-                               out[1].data_ptr(), _stream(key_cache), tokens, code)
+                               out[1].data_ptr(), _stream_on(device), tokens, code)
     _call_on(device, "nml_sm100_paged_read_q8", request)
     return out
 
@@ -761,7 +767,7 @@ def paged_attention_q8(query: torch.Tensor, key_cache: torch.Tensor, key_scales:
         return out
     request = _abi.PagedAttentionQ8(
         0, cache, query.data_ptr(), _ptr(query_offsets), _ptr(sinks), out.data_ptr(), None, 0,
-        _stream(query), tokens, heads, *strides, sliding_window or 0, first_tokens, splits or 0,
+        _stream_on(device), tokens, heads, *strides, sliding_window or 0, first_tokens, splits or 0,
         dim ** -0.5 if scale is None else scale, code)
     request.struct_size = ctypes.sizeof(request)
     size = _abi.load().nml_sm100_paged_attention_q8_workspace_bytes(ctypes.byref(request))
