@@ -167,34 +167,30 @@ row_kernel(const AttentionParams p) {
       words[w + 2][0] = hi.x; words[w + 2][1] = hi.y; words[w + 3][0] = hi.z;
       words[w + 3][1] = hi.w;
     }
-    float inverse = 1.0f;
-    if constexpr (std::is_same<T, __half>::value) {
+    uint32_t largest = 0;  // magnitude bits in the upper half
 #pragma unroll
-      for (int w = 0; w < KW; ++w) {
-        q[n][w][0] = words[w][0];
-        q[n][w][1] = words[w][1];
+    for (int w = 0; w < KW; ++w) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        largest = max(largest, max((words[w][i] & 0x7fffu) << 16, words[w][i] & 0x7fff0000u));
       }
-    } else {
-      uint32_t largest = 0;
+    }
+    largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+    largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    const int shift = kHalf ? 0 : query_shift(largest);
+    const float up = exp2_int(shift);
+    // a query with an infinity or a NaN gives NaN
+    const float inverse = largest >= (kHalf ? 0x7c000000u : 0x7f800000u)
+                              ? __uint_as_float(0x7fc00000u)
+                              : exp2_int(-shift);
 #pragma unroll
-      for (int w = 0; w < KW; ++w) {
+    for (int w = 0; w < KW; ++w) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          largest = max(largest, max((words[w][i] & 0x7fffu) << 16, words[w][i] & 0x7fff0000u));
-        }
-      }
-      largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-      largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-      const int shift = query_shift(largest);
-      const float up = exp2_int(shift);
-      inverse = exp2_int(-shift);
-#pragma unroll
-      for (int w = 0; w < KW; ++w) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          q[n][w][i] = Elem<__half>::pack2(Elem<T>::from_bits(words[w][i] & 0xffffu) * up,
-                                           Elem<T>::from_bits(words[w][i] >> 16) * up);
-        }
+      for (int i = 0; i < 2; ++i) {
+        q[n][w][i] = kHalf ? words[w][i]
+                           : Elem<__half>::pack2(Elem<T>::from_bits(words[w][i] & 0xffffu) * up,
+                                                 Elem<T>::from_bits(words[w][i] >> 16) * up);
       }
     }
     factor[n][0] = p.scale_log2 * __shfl_sync(0xffffffffu, inverse, 8 * c);
@@ -721,8 +717,10 @@ extern "C" int32_t nml_sm100_paged_attention_q8(const NmlSm100PagedAttentionQ8* 
   p.group = static_cast<int>(r.query_heads / r.cache.kv_heads);
   p.head_tiles = p.group <= 8 ? 1 : (p.group + 15) / 16;
   p.splits = static_cast<int>(splits);
-  p.window = static_cast<int>(r.sliding_window);
-  p.first = static_cast<int>(r.first_tokens);
+  // no sequence is longer than its table
+  const int64_t longest = r.cache.table_width * kCachePage;
+  p.window = r.sliding_window < longest ? static_cast<int>(r.sliding_window) : 0;
+  p.first = static_cast<int>(r.first_tokens < longest ? r.first_tokens : longest);
   p.scale_log2 = r.scale * kLog2e;
   p.status = device->status_word;
   cudaStream_t stream = static_cast<cudaStream_t>(r.stream);

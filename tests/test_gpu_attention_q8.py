@@ -144,6 +144,55 @@ def test_nan_tokens_reach_only_rows_that_see_them(dim):
         ref.assert_attention_close(one, expected, bound, torch.bfloat16)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("runs", [False, True])
+@pytest.mark.parametrize("splits", [1, 3])
+def test_queries_that_are_not_finite(dtype, runs, splits):
+    new, before = ([20, 9], [300, 140]) if runs else ([1, 1], [319, 148])
+    lengths, table, cache, query, sinks, offsets = make(13, dtype, 64, 2, 8, new, before)
+    query[0, 3, 5] = float("inf")
+    query[-1, 9, 63] = -float("inf")
+    query[-1, 14, 0] = float("nan")
+    out = call(query, cache, table, lengths, offsets if runs else None, None, splits=splits)
+    assert status() == 0
+    bad = ~torch.isfinite(query).all(-1)
+    expected, bound = ref.attention(torch.where(bad[..., None], 0, query), cache, table, lengths,
+                                    offsets, None, 0, 0, 0.125)
+    expected[bad] = float("nan")
+    ref.assert_attention_close(out, expected, bound, dtype)
+
+
+@pytest.mark.parametrize("runs", [False, True])
+def test_windows_past_every_length(runs):
+    """The largest windows and counts of first tokens that the call takes."""
+    most = 2 ** 31 - 1
+    new, before = ([70, 3], [40, 200]) if runs else ([1, 1], [109, 202])
+    lengths, table, cache, query, sinks, offsets = make(14, torch.bfloat16, 64, 1, 8, new, before)
+    given = offsets if runs else None
+    plain = call(query, cache, table, lengths, given, None)
+    assert torch.equal(call(query, cache, table, lengths, given, None, sliding_window=most), plain)
+    wide = call(query, cache, table, lengths, given, None, sliding_window=5,
+                first_tokens=most - 16)
+    assert status() == 0
+    expected, bound = ref.attention(query, cache, table, lengths, offsets, None, 5, 10 ** 6, 0.125)
+    ref.assert_attention_close(wide, expected, bound, torch.bfloat16)
+
+
+def test_nothing_to_do():
+    """No rows, a batch of empty places, sequences without rows."""
+    lengths, table, cache, query, _, _ = make(15, torch.bfloat16, 64, 2, 8, [4, 4], [0, 30])
+    assert call(query[:0], cache, table, lengths, [0, 0, 0], None).shape == (0, 16, 64)
+    assert (call(query[:2], cache, table, [0, 0], None, None) == 0).all()
+    from nml_b200 import ops
+    out = torch.full((8, 16, 64), 3.0, dtype=torch.bfloat16, device="cuda")
+    for splits in (1, 2):
+        ops.paged_attention_q8(query.cuda(), *[x.cuda() for x in cache], table.cuda(),
+                               torch.tensor(lengths, dtype=torch.int32).cuda(),
+                               query_offsets=torch.tensor([3, 3, 3], dtype=torch.int32).cuda(),
+                               splits=splits, out=out)
+        assert status() == 0 and (out == 3).all()
+
+
 @pytest.mark.parametrize("splits", [1, 4])
 def test_rows_outside_every_sequence_stay(splits):
     lengths, table, cache, query, sinks, _ = make(5, torch.float16, 64, 2, 8, [3, 0, 40, 9],

@@ -248,3 +248,57 @@ def test_cache_past_32_bit_offsets():
                                         0, 0, dim ** -0.5)
         ref.assert_attention_close(out, expected, bound, torch.float16)
     assert back[0].shape == (length, kv_heads, dim)
+
+
+def test_appends_in_graphs_and_on_two_streams():
+    """A captured append replayed with new rows, beside an eager one on another stream."""
+    from nml_b200 import ops
+    gen = torch.Generator().manual_seed(9)
+    kv_heads, dim, lengths = 2, 64, [40, 7, 200]
+    table, pages = ref.random_table(gen, lengths)
+    caches = [to_device(ref.random_cache(gen, pages, kv_heads, dim)) for _ in range(2)]
+    before = [[x.cpu() for x in cache] for cache in caches]
+    rows = [make_rows(gen, 3, kv_heads, dim, torch.bfloat16) for _ in range(2)]
+    given = torch.zeros((3, kv_heads, dim), dtype=torch.bfloat16, device="cuda")
+    arguments = (table.cuda(), torch.tensor(lengths, dtype=torch.int32).cuda())
+    kept = [x.clone() for x in caches[0]]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        query = ops.paged_append_q8(given, given, *caches[0], *arguments, query=given)
+    for cache, old in zip(caches[0], kept):  # capturing runs nothing
+        assert torch.equal(cache, old)
+    given.copy_(rows[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.paged_append_q8(rows[1].cuda(), rows[1].cuda(), *caches[1], *arguments)
+    graph.replay()
+    assert status() == 0
+    assert torch.equal(query.cpu(), rows[0])
+    for cache, old, new in zip(caches, before, rows):
+        for at in (0, 2):
+            want = ref.append(new.double(), old[at], old[at + 1], table, lengths, [0, 1, 2, 3])
+            assert torch.equal(cache[at].cpu(), want[0])
+            assert torch.equal(cache[at + 1].cpu(), want[1])
+
+
+def test_appending_and_reading_nothing():
+    from nml_b200 import ops
+    gen = torch.Generator().manual_seed(10)
+    table, pages = ref.random_table(gen, [20, 20])
+    cache = ref.random_cache(gen, pages, 2, 64)
+    dev = to_device(cache)
+    rows = torch.ones((2, 2, 64), dtype=torch.float16, device="cuda")
+    none = torch.zeros(2, dtype=torch.int32, device="cuda")
+    assert ops.paged_append_q8(rows, rows, *dev, table.cuda(), none) is None
+    empty = torch.zeros(3, dtype=torch.int32, device="cuda")
+    lengths = torch.tensor([20, 20], dtype=torch.int32, device="cuda")
+    out = ops.paged_append_q8(rows[:0], rows[:0], *dev, table.cuda(), lengths, empty,
+                              query=rows[:0])
+    assert out.shape == (0, 2, 64)
+    ops.paged_append_q8(rows, rows, *dev, table.cuda(), lengths, empty)
+    key, value = ops.paged_read_q8(*dev, table.cuda(), empty, 0)
+    assert key.shape == value.shape == (0, 2, 64)
+    assert status() == 0
+    for got, want in zip(dev, cache):
+        assert torch.equal(got.cpu(), want)
