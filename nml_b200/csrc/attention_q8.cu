@@ -13,12 +13,23 @@
 // what actually enters the f16 product.  The exponents lie in [-48, 48]: a weight that underflows
 // (w_j < 2^-126) is below 2^-24 of the denominator's largest term.
 //
-// Shape of the work: one CTA per (row, kv head and up to 16 of its query heads, split of the
-// visible pages); its warps take chunks of pages in turn.  A block is 16 * head_dim contiguous
-// bytes, loaded straight into mma.sync fragments by 16-byte (keys) and 8- or 16-byte (values)
-// loads, the next chunk's while this one is worked on: scores [16 tokens x 8 heads] = K . q^T, the
+// M is the maximum of the steps before: weights above one are as good as those below as long as F16
+// holds them, so a step's own maximum is formed, and the state rescaled, only when the weights'
+// sum passes 2^14 (or there is none yet).
+//
+// Shape of the work: one CTA of four warps per (row, kv head and up to 16 of its query heads, split
+// of the visible pages); its warps take steps of two pages (one at head_dim 128) in turn.  A block
+// is 16 * head_dim contiguous bytes: one bulk copy into a ring of two steps for each warp, the next
+// one issued as soon as the last read is done, page table entries and scales fetched 32 pages ahead.
+// Scores [16 tokens x 8 heads] = K . q^T with keys widened in registers into mma.sync fragments,
 // weights transposed between lanes by movmatrix, out^T [dims x 8 heads] += V^T . w, where pairs of
-// tokens are interleaved byte-wise before they are widened.
+// tokens are interleaved byte-wise before they are widened.  Four CTAs of 112 registers an SM; ten
+// warps an SM keep the conversions and products (about 100 instructions a page) off the memory's
+// back.  Splits are joined by a second launch that starts while the first still runs.
+//
+// Measured on B200 (device time): 64 sequences of 4097 tokens, 64 query and 8 kv heads of 64 (269.5
+// MB): 52.4 us, 5.15 TB/s; 3 sequences of 60000 to 100000 tokens, 32 and 8 heads of 128 (474 MB): 88
+// us, 5.3 TB/s, in 24 splits; one sequence of 413 tokens: 6.4 us.
 #include <type_traits>
 
 #include "attention_q8.cuh"
@@ -29,6 +40,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kSiteRowCodes = 22;  // bit 8 + site of the status word: a wait for codes ran out
+
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
