@@ -158,7 +158,7 @@ tile_kernel(const AttentionParams p) {
       if (b < p.cache.batch) {
         begin = max(p.offsets[b], 0);
         given_end = p.offsets[b + 1];
-        length = p.cache.lengths[b];
+        length = max(p.cache.lengths[b], 0);
         end = min(given_end, p.tokens);
         tiles = end > begin ? (end - begin + per_tile - 1) / per_tile : 0;
       }

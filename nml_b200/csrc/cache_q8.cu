@@ -157,7 +157,7 @@ append_kernel(const AppendParams p) {
         const int begin = p.offsets == nullptr ? row : p.offsets[sequence];
         const int given_end = p.offsets == nullptr ? row + 1 : p.offsets[sequence + 1];
         const int end = min(given_end, p.tokens);
-        position = p.cache.lengths[sequence] - given_end + row;
+        position = max(p.cache.lengths[sequence], 0) - given_end + row;
         const int limit = p.cache.table_width * kCachePage;
         const int usable = p.rotary == nullptr ? limit : min(limit, p.rotary_rows);
         if (position >= usable) {
@@ -332,7 +332,7 @@ read_kernel(const ReadParams p) {
       if (sequence >= 0) {
         const int position = row - p.offsets[sequence];
         source = -1;
-        if (position >= p.cache.table_width * kCachePage) {
+        if (position < 0 || position >= p.cache.table_width * kCachePage) {
           atomicOr(p.status, NML_SM100_STATUS_INDEX_RANGE);
         } else {
           const int page = physical_page(p.cache, sequence, position / kCachePage, p.status);

@@ -74,9 +74,10 @@ __device__ __forceinline__ int physical_page(const CacheQ8& cache, int sequence,
   return page;
 }
 
-// Tokens of a sequence that its table can address; more raise the status bit.
+// Tokens of a sequence that its table can address; more raise the status bit, fewer than none are
+// none.
 __device__ __forceinline__ int sequence_length(const CacheQ8& cache, int sequence, int* status) {
-  const int length = cache.lengths[sequence];
+  const int length = max(cache.lengths[sequence], 0);
   if (length > cache.table_width * kCachePage) {
     atomicOr(status, NML_SM100_STATUS_INDEX_RANGE);
     return cache.table_width * kCachePage;

@@ -178,6 +178,17 @@ def test_windows_past_every_length(runs):
     ref.assert_attention_close(wide, expected, bound, torch.bfloat16)
 
 
+@pytest.mark.parametrize("runs", [False, True])
+def test_lengths_below_zero_are_empty(runs):
+    new = [5, 4] if runs else [1, 1]
+    lengths, table, cache, query, _, offsets = make(16, torch.bfloat16, 64, 2, 8, new, [20, 30])
+    given = offsets if runs else None
+    want = call(query, cache, table, [0, lengths[1]], given, None)
+    for empty in (-1, -2 ** 31):
+        assert torch.equal(call(query, cache, table, [empty, lengths[1]], given, None), want)
+    assert status() == 0 and (want[: new[0]] == 0).all()
+
+
 def test_nothing_to_do():
     """No rows, a batch of empty places, sequences without rows."""
     lengths, table, cache, query, _, _ = make(15, torch.bfloat16, 64, 2, 8, [4, 4], [0, 30])

@@ -133,8 +133,8 @@ def test_append_leaves_what_is_not_its_own():
     """Empty places of a padded batch, rows outside every sequence, pages of other sequences."""
     from nml_b200 import ops
     gen = torch.Generator().manual_seed(5)
-    kv_heads, dim, lengths = 2, 64, [17, 0, 3, 0]
-    table, pages = ref.random_table(gen, lengths)
+    kv_heads, dim, lengths = 2, 64, [17, 0, 3, -2 ** 31]
+    table, pages = ref.random_table(gen, [17, 0, 3, 0])
     cache = ref.random_cache(gen, pages, kv_heads, dim)
     dev = to_device(cache)
     rows = make_rows(gen, 4, kv_heads, dim, torch.bfloat16)
