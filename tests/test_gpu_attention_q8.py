@@ -82,6 +82,14 @@ RUNS = [
     (128, 2, 4, [140, 60], [3, 200], 0, 0, True),
     (128, 1, 8, [100, 1], [0, 260], 64, 5, False),
     (128, 1, 5, [70], [0], 0, 0, False),
+    # short runs: a few rows that share what is read of their sequence
+    (64, 2, 8, [4, 1, 0, 3, 9], [100, 0, 20, 1500, 37], 0, 0, True),
+    (64, 1, 5, [5, 5, 2], [3, 200, 14], 64, 2, False),
+    (64, 3, 1, [3, 8], [700, 13], 0, 0, True),
+    (64, 1, 8, [5, 4], [126, 60], 16, 20, False),
+    (128, 2, 4, [2, 3, 1], [130, 0, 900], 0, 0, True),
+    (128, 1, 8, [5, 0, 4], [15, 3, 400], 33, 1, False),
+    (64, 1, 16, [2, 2], [500, 30], 0, 0, False),
 ]
 
 
@@ -142,6 +150,27 @@ def test_nan_tokens_reach_only_rows_that_see_them(dim):
                                         dim ** -0.5)
         assert expected.isnan().any() == (window == 0)
         ref.assert_attention_close(one, expected, bound, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("splits", [1, 2])
+def test_nan_tokens_in_short_runs(dim, splits):
+    """The same for the rows of a short run: values that are NaN inside the run itself and, past a
+    window, in front of some of its rows."""
+    # row i is at position 200 + i: a window of 8 ends before row 195 + 8 - 200 = 3
+    for window, token, first_nan, last_nan in ((0, 201, 1, 5), (8, 195, 0, 3), (8, 203, 3, 5)):
+        lengths, table, cache, query, _, offsets = make(17, torch.bfloat16, dim, 2, 8, [5], [200])
+        page, slot = int(table[0, token // 16]), token % 16
+        cache[2][page, 1, slot] = 0x7f   # a value row of head 1
+        cache[0][page, 0, slot] = 0xff   # a key row of head 0
+        out = call(query, cache, table, lengths, offsets, None, sliding_window=window or None,
+                   splits=splits)
+        assert status() == 0
+        expected, bound = ref.attention(query, cache, table, lengths, offsets, None, window, 0,
+                                        dim ** -0.5)
+        rows = expected.isnan().any(-1).all(-1)
+        assert rows.tolist() == [first_nan <= i < last_nan for i in range(5)]
+        ref.assert_attention_close(out, expected, bound, torch.bfloat16)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
