@@ -500,12 +500,12 @@ join_kernel(const AttentionParams p) {
   const int64_t query_head = static_cast<int64_t>(blockIdx.x) * kHeads + warp / kJoinWarps;
   const int row = static_cast<int>(query_head / p.query_heads);
   // (a CTA of one head leaves as a whole)
-  if (row >= p.tokens ||
-      (p.offsets != nullptr && sequence_of_row(p.offsets, p.cache.batch, row) < 0)) {
-    return;
-  }
-  // launched while the splits still run: everything above overlaps with them
+  const bool nobodys = row >= p.tokens || (p.offsets != nullptr &&
+                                           sequence_of_row(p.offsets, p.cache.batch, row) < 0);
+  // Launched while the splits still run: everything above overlaps with them.  Every CTA waits, so
+  // that this launch never ends before the one that it belongs to.
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (nobodys) return;
   const float* base = p.partial + query_head * p.splits * kStride;
   float total_max = -INFINITY;
   for (int s = lane; s < p.splits; s += 32) total_max = fmaxf(total_max, base[s * kStride + D]);
