@@ -302,3 +302,32 @@ def test_appending_and_reading_nothing():
     assert status() == 0
     for got, want in zip(dev, cache):
         assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new", [1, 60])
+def test_blocks_that_grow_are_moved_whole(dim, new):
+    """Every sequence's partly filled block grows its exponent: all lanes of the warp that moves the
+    older codes go by the exponent from before the call, each time."""
+    from nml_b200 import ops
+    gen = torch.Generator().manual_seed(19 + new)
+    kv_heads, batch = 4, 24
+    counts, before = [new] * batch, [1 + i % 15 for i in range(batch)]
+    lengths = [n + m for n, m in zip(counts, before)]
+    table, pages = ref.random_table(gen, lengths)
+    cache = ref.random_cache(gen, pages, kv_heads, dim)
+    offsets, tokens = ref.offsets_of(counts), sum(counts)
+    rows = [make_rows(gen, tokens, kv_heads, dim, torch.bfloat16) for _ in range(2)]
+    for x in rows:
+        x[offsets[:-1]] *= (2.0 ** (1 + torch.arange(batch) % 7))[:, None, None]
+    expected = [*ref.append(rows[0].double(), cache[0], cache[1], table, lengths, offsets),
+                *ref.append(rows[1].double(), cache[2], cache[3], table, lengths, offsets)]
+    arguments = [table.cuda(), torch.tensor(lengths, dtype=torch.int32).cuda(),
+                 torch.tensor(offsets, dtype=torch.int32).cuda()]
+    start, rows = to_device(cache), to_device(rows)
+    for _ in range(20):
+        dev = [x.clone() for x in start]
+        ops.paged_append_q8(*rows, *dev, *arguments)
+        for got, want in zip(dev, expected):
+            assert torch.equal(got.cpu(), want)
+    assert status() == 0
