@@ -573,6 +573,7 @@ tile_kernel(const AttentionParams p) {
           }
           control.pages[j % kInfoSteps][lane] = info;
         }
+        __syncwarp();  // lane 0's arrival hands over the other lanes' page data too
         const uint32_t there = __ballot_sync(0xffffffffu, mine && held >= 0);
         if (lane == 0) {
           mbar_arrive_expect_tx(&control.staged_full[slot], __popc(there) * 2 * kBlockBytes);

@@ -377,3 +377,18 @@ def test_prompts_and_tokens_in_a_row():
                 limit = written[b].abs() * 2.0 ** -4 * 1.07 + \
                     2 * 2.0 ** -10 * torch.exp2(exponent)[..., None]
                 assert ((value - written[b]).abs() <= limit).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_runs_repeat_themselves(dim):
+    """Every step goes by its own pages' scales: magnitudes that change from page to page, many tiles
+    beside each other, the same bits each time."""
+    new, before = [90, 33, 150, 64] * 3, [400, 900, 0, 77] * 3
+    lengths, table, cache, query, sinks, offsets = make(21, torch.bfloat16, dim, 2, 8, new, before,
+                                                        spread=3.0, with_sinks=True)
+    out = call(query, cache, table, lengths, offsets, sinks)
+    expected, bound = ref.attention(query, cache, table, lengths, offsets, sinks, 0, 0, dim ** -0.5)
+    ref.assert_attention_close(out, expected, bound, torch.bfloat16)
+    for _ in range(20):
+        assert torch.equal(call(query, cache, table, lengths, offsets, sinks), out)
+    assert status() == 0
