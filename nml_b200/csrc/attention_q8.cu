@@ -292,6 +292,8 @@ row_kernel(const AttentionParams p) {
         for (int n = 0; n < NT; ++n) {
           if (!seen_g) s[n][i][0] = s[n][i][1] = -INFINITY;
           if (!seen_h) s[n][i][2] = s[n][i][3] = -INFINITY;
+          score_factor[n][i][0] = masked_factor(score_factor[n][i][0]);
+          score_factor[n][i][1] = masked_factor(score_factor[n][i][1]);
         }
       }
     }

@@ -35,6 +35,13 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return r;
 }
 
+// A factor of scores among which are masked ones, -infinity: what rounds to zero (a query row below
+// 2^-85 or a tiny scale, times the factor of a block of zero keys, 2^-48) would make NaN of them.
+// Scores are below 2^32, so that a factor of 2^-126 changes no weight.
+__device__ __forceinline__ float masked_factor(float factor) {
+  return factor < 1.1754944e-38f ? 1.1754944e-38f : factor;
+}
+
 // Power of two that puts the largest magnitude of a BF16 row (given as f32 bits) into
 // [2^14, 2^15), so that the row's narrowing to F16 is exact down to 2^-29 of it; none for rows of
 // zeros or with an infinity or a NaN.

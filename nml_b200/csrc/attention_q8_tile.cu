@@ -389,6 +389,8 @@ tile_kernel(const AttentionParams p) {
           for (int i = 0; i < kStepTokens; ++i) {
             if ((seen[i / 32] >> (i % 32) & 1u) == 0) s[i] = -INFINITY;
           }
+#pragma unroll
+          for (int q = 0; q < kStepPages; ++q) page_factor[q] = masked_factor(page_factor[q]);
           __syncwarp();
         }
         if (with_maximum) {

@@ -392,3 +392,42 @@ def test_runs_repeat_themselves(dim):
     for _ in range(20):
         assert torch.equal(call(query, cache, table, lengths, offsets, sinks), out)
     assert status() == 0
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("splits", [1, 2])
+@pytest.mark.parametrize("runs", [False, True])
+def test_masked_tokens_of_tiny_scores(dim, runs, splits):
+    """A score factor below f32's smallest number (tiny queries, or a tiny scale, over blocks of zero
+    keys, whose exponent is the least) leaves what is masked out masked: the seen values' mean."""
+    new, before = ([40, 9], [60, 140]) if runs else ([1, 1], [99, 148])
+    given = None
+    for dtype, magnitude, scale in ((torch.bfloat16, 2.0 ** -90, None), (torch.bfloat16, 1.0, 1e-36),
+                                    (torch.float16, 1.0, 1e-36), (torch.bfloat16, 2.0 ** -126, 1e-38)):
+        lengths, table, cache, query, sinks, offsets = make(22, dtype, dim, 2, 8, new, before)
+        cache[0].zero_()
+        cache[1].fill_(127 - 48)
+        query = (query.float() * magnitude).to(dtype)
+        given = offsets if runs else None
+        for window in (0, 37):
+            out = call(query, cache, table, lengths, given, None, scale=scale, splits=splits,
+                       sliding_window=window or None)
+            assert status() == 0
+            expected, bound = ref.attention(query, cache, table, lengths, offsets, None, window, 0,
+                                            dim ** -0.5 if scale is None else scale)
+            assert torch.isfinite(expected).all()
+            ref.assert_attention_close(out, expected, bound, dtype)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("group", [1, 8])
+def test_many_more_rows_than_tokens(dim, group):
+    """Rows up to 100 positions in front of the first token share a tile with rows that see some."""
+    lengths, table, cache, query, _, offsets = make(23, torch.bfloat16, dim, 2, group, [120, 50],
+                                                    [0, 0])
+    lengths = [20, 41]
+    out = call(query, cache, table, lengths, offsets, None)
+    assert status() == 0
+    expected, bound = ref.attention(query, cache, table, lengths, offsets, None, 0, 0, dim ** -0.5)
+    assert (expected[:100] == 0).all() and (expected[120:129] == 0).all()
+    ref.assert_attention_close(out, expected, bound, torch.bfloat16)
