@@ -679,8 +679,9 @@ int32_t nml_sm100_paged_read_q8(const NmlSm100PagedReadQ8 *request, char *error_
  * tokens): rows [query_offsets[b], query_offsets[b + 1]) are the last tokens of sequence b, as in
  * the append.  Token j is visible at position i when j <= i and, with a sliding window,
  * j > i - sliding_window or j < first_tokens.  `sinks` as in the 16-bit operator.  A row that sees
- * nothing becomes zeros; rows outside every sequence are left as they were.  A row with an infinity
- * or a NaN among its queries, or that sees a token stored as NaN, becomes NaN.  Scores, softmax
+ * nothing becomes zeros, whatever its queries hold; rows outside every sequence are left as they
+ * were.  A row that sees a token becomes NaN when its queries hold an infinity or a NaN, or when a
+ * token that it sees is stored as NaN.  Scores, softmax
  * statistics and sums are f32; queries of BF16 are narrowed to F16 after a power of two for every
  * row that makes this exact down to 2^-29 of the row's largest; probabilities are narrowed to F16. */
 typedef struct NmlSm100PagedAttentionQ8 {

@@ -161,6 +161,7 @@ row_kernel(const AttentionParams p) {
   // (word w of a token: dimensions 64 (w / 4) + 16 c + 4 (w % 4) .. + 3).
   uint32_t q[NT][KW][2];
   float factor[NT][2];  // scale * log2(e) / (the row's power of two) of heads 2c and 2c + 1
+  uint32_t poisoned = 0;  // bit 2n + j: head 2c + j's query holds an infinity or a NaN
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int head = head_base + 8 * n + g;
@@ -192,14 +193,14 @@ row_kernel(const AttentionParams p) {
     constexpr bool kHalf = std::is_same<T, __half>::value;
     const int shift = kHalf ? 0 : query_shift(largest);
     const float up = exp2_int(shift);
-    // a query with an infinity or a NaN gives NaN
-    const float inverse = largest >= (kHalf ? 0x7c000000u : 0x7f800000u)
-                              ? __uint_as_float(0x7fc00000u)
-                              : exp2_int(-shift);
+    // a query with an infinity or a NaN gives NaN where it sees a token; its scores are not formed
+    const bool bad = largest >= (kHalf ? 0x7c000000u : 0x7f800000u);
+    const float inverse = exp2_int(-shift);
 #pragma unroll
     for (int w = 0; w < KW; ++w) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
+        if (bad) words[w][i] = 0;
         q[n][w][i] = kHalf ? words[w][i]
                            : Elem<__half>::pack2(Elem<T>::from_bits(words[w][i] & 0xffffu) * up,
                                                  Elem<T>::from_bits(words[w][i] >> 16) * up);
@@ -207,6 +208,8 @@ row_kernel(const AttentionParams p) {
     }
     factor[n][0] = p.scale_log2 * __shfl_sync(0xffffffffu, inverse, 8 * c);
     factor[n][1] = p.scale_log2 * __shfl_sync(0xffffffffu, inverse, 8 * c + 4);
+    const uint32_t bad_lanes = __ballot_sync(0xffffffffu, bad);
+    poisoned |= (bad_lanes >> (8 * c) & 1u) << (2 * n) | (bad_lanes >> (8 * c + 4) & 1u) << (2 * n + 1);
   }
 
   float running_max[NT][2], running_sum[NT][2];
@@ -439,6 +442,9 @@ row_kernel(const AttentionParams p) {
       sum += __shfl_xor_sync(0xffffffffu, sum, 4);
       sum += __shfl_xor_sync(0xffffffffu, sum, 8);
       sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+      if ((poisoned >> (2 * n + j) & 1u) != 0 && running_max[n][j] != -INFINITY) {
+        sum = __uint_as_float(0x7fc00000u);
+      }
       float* state = merged[warp][8 * n + 2 * c + j];
 #pragma unroll
       for (int i = 0; i < 2 * VW; ++i) {

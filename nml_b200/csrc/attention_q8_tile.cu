@@ -476,9 +476,12 @@ tile_kernel(const AttentionParams p) {
       tcgen05_fence_after_sync();
     }
     const int64_t query_head = static_cast<int64_t>(first_row + token) * p.query_heads + head;
-    // a row that sees nothing has no maximum; its output is zero
-    if (running_max == -INFINITY) running_sum = 0.0f;
-    if (poisoned) running_sum = __uint_as_float(0x7fc00000u);
+    // a row that sees nothing has no maximum; its output is zero, whatever its queries hold
+    if (running_max == -INFINITY) {
+      running_sum = 0.0f;
+    } else if (poisoned) {
+      running_sum = __uint_as_float(0x7fc00000u);
+    }
     float denominator = running_sum;
     if (p.sinks != nullptr && live) {
       denominator += exp2f(sink - running_max);

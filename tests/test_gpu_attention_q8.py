@@ -431,3 +431,32 @@ def test_many_more_rows_than_tokens(dim, group):
     expected, bound = ref.attention(query, cache, table, lengths, offsets, None, 0, 0, dim ** -0.5)
     assert (expected[:100] == 0).all() and (expected[120:129] == 0).all()
     ref.assert_attention_close(out, expected, bound, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("splits", [1, 2])
+@pytest.mark.parametrize("runs", [False, True])
+def test_queries_that_are_not_finite_and_see_nothing(dtype, runs, splits):
+    """Empty places of a padded batch, rows in front of the first token and rows whose only page is
+    bad give zeros whatever their queries hold, in either kernel."""
+    from nml_b200 import _abi
+    new, before = ([5, 30, 4, 7], [0, 0, 40, 0]) if runs else ([1, 1, 1, 1], [0, 0, 43, 0])
+    lengths, table, cache, query, _, offsets = make(24, dtype, 64, 2, 8, new, before)
+    lengths[:2] = [0, 12 if runs else 0]
+    given = offsets if runs else None
+    query[:, 1::2] = float("nan")
+    query[:, 4] = float("inf")
+    bad = ~torch.isfinite(query).all(-1)
+    expected, bound = ref.attention(torch.where(bad[..., None], 0, query), cache, table, lengths,
+                                    offsets, None, 0, 0, 0.125)
+    sees = torch.cat([torch.arange(n) + m - n >= 0 for n, m in zip(new, lengths)])
+    expected[bad & sees[:, None]] = float("nan")
+    out = call(query, cache, table, lengths, given, None, splits=splits)
+    assert status() == 0
+    assert (out[~sees.cuda()] == 0).all()
+    ref.assert_attention_close(out, expected, bound, dtype)
+    table[3] = -1  # nothing of the last sequence can be seen
+    out = call(query, cache, table, lengths, given, None, splits=splits)
+    assert status() == _abi.STATUS_INDEX_RANGE
+    assert (out[offsets[3]:] == 0).all()
+    ref.assert_attention_close(out[:offsets[3]], expected[:offsets[3]], bound[:offsets[3]], dtype)
