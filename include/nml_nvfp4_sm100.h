@@ -592,7 +592,8 @@ size_t nml_sm100_paged_attention_decode_workspace_bytes(int64_t batch, int64_t q
  *   codes   u8 [physical_pages, kv_heads, page_size, head_dim]
  *   scales  u8 [physical_pages, kv_heads], E8M0: value = e4m3(code) * 2^(scale - 127)
  * so that a block is contiguous (1 or 2 KB).  Not part of the reference: its caches hold 16-bit
- * values (crates/nml-ir/src/lib.rs:4717-4730).  Limits: head_dim 64 or 128, page_size 16.
+ * values (crates/nml-ir/src/lib.rs:4717-4730).  Limits: head_dim 64 or 128, page_size 16, tables of
+ * less than 2^27 - 64 pages.
  *
  * Quantisation: the exponent of a block is the smallest e in [-48, 48] with |x| <= 448 * 2^e for
  * every finite row written to it, codes round to nearest even, larger magnitudes saturate.  A

@@ -99,7 +99,8 @@ row_kernel(const AttentionParams p) {
   if (sequence < 0) return;  // a row of no sequence is left as it was
   int length = sequence_length(p.cache, sequence, p.status);
   if (p.offsets != nullptr) length += row + 1 - p.offsets[sequence + 1];
-  const Visible v = visible_pages(length, p.window > 0 ? length - p.window : 0, p.first);
+  const Visible v = visible_pages(length, p.window > 0 ? length - p.window : 0, p.first,
+                                  p.cache.table_width * kCachePage);
   const int per_split = (v.pages + p.splits - 1) / p.splits;
   const int page_begin = split * per_split;
   const int page_end = min(v.pages, page_begin + per_split);

@@ -52,15 +52,16 @@ __device__ __forceinline__ int query_shift(uint32_t largest_bits) {
 
 // Which logical pages queries see: [0, front) and [back, end), of `pages` entries in this order.
 struct Visible {
-  int length;  // tokens in front of (and with) the last query's own
+  int length;  // tokens in front of (and with) the last query's own, those of the table
   int start;   // first token of the first query's window
   int front, back, pages;
 };
 
-__device__ __forceinline__ Visible visible_pages(int length, int start, int first) {
+// `most`: tokens that the sequence's table can address; positions may lie past them.
+__device__ __forceinline__ Visible visible_pages(int length, int start, int first, int most) {
   Visible v;
-  v.length = max(length, 0);
-  v.start = max(start, 0);
+  v.length = min(max(length, 0), most);
+  v.start = min(max(start, 0), v.length);
   const int end = (v.length + kCachePage - 1) / kCachePage;
   v.back = min(v.start / kCachePage, end);
   v.front = v.start > 0 ? min((first + kCachePage - 1) / kCachePage, v.back) : 0;

@@ -181,10 +181,8 @@ tile_kernel(const AttentionParams p) {
       passed += __shfl_sync(0xffffffffu, upto, 31);
     }
     if (lane == 0) {
-      const int most = p.cache.table_width * kCachePage;
-      if (sequence >= 0 && length > most) {
+      if (sequence >= 0 && length > p.cache.table_width * kCachePage) {
         atomicOr(p.status, NML_SM100_STATUS_INDEX_RANGE);
-        length = most;
       }
       control.sequence = sequence;
       control.first_row = begin + tile * per_tile;
@@ -217,8 +215,9 @@ tile_kernel(const AttentionParams p) {
 
   const int first_row = control.first_row, rows = control.rows;
   const int first_position = control.first_position;
+  const int most = p.cache.table_width * kCachePage;
   const Visible v = visible_pages(first_position + rows,
-                                  p.window > 0 ? first_position + 1 - p.window : 0, p.first);
+                                  p.window > 0 ? first_position + 1 - p.window : 0, p.first, most);
   const int all_steps = (v.pages + kStepPages - 1) / kStepPages;
   const int per_split = (all_steps + p.splits - 1) / p.splits;
   const int step_begin = min(all_steps, split * per_split);
@@ -269,8 +268,9 @@ tile_kernel(const AttentionParams p) {
     take_registers<S::kSoftmaxRegisters>();
     const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
     // rows of nobody walk like the last row, so that they do not ask for masks
-    const int length = first_position + 1 + (live ? token : rows - 1);
-    const int start = p.window > 0 ? max(0, length - p.window) : 0;
+    const int position = first_position + (live ? token : rows - 1);
+    const int length = min(position + 1, most);
+    const int start = p.window > 0 ? min(max(0, position + 1 - p.window), most) : 0;
 
     // q: largest magnitude, then F16 into tensor memory, column c holding elements 2c and 2c + 1
     float factor = p.scale_log2;
@@ -318,10 +318,10 @@ tile_kernel(const AttentionParams p) {
 
     // steps whose tokens every row of the tile sees: behind the last row's window start, in front
     // of the first row's own token
-    const int last_start = p.window > 0 ? max(0, first_position + rows - p.window) : 0;
+    const int last_start = p.window > 0 ? min(max(0, first_position + rows - p.window), most) : 0;
     const int first_whole = last_start == 0 ? 0 : v.front + (last_start + kCachePage - 1) /
                                                                 kCachePage - v.back;
-    const int whole_pages = v.front + max(first_position + 1, 0) / kCachePage - v.back;
+    const int whole_pages = v.front + min(max(first_position + 1, 0), most) / kCachePage - v.back;
     const int whole_begin = (first_whole + kStepPages - 1) / kStepPages - step_begin;
     const int whole_end = max(whole_pages, 0) / kStepPages - step_begin;
 

@@ -25,7 +25,8 @@ inline bool valid_cache_q8(const NmlSm100CacheQ8& c, bool lengths) {
          (!lengths || c.sequence_lengths != nullptr) && fits_i32(c.batch) &&
          fits_i32(c.kv_heads) && fits_i32(c.physical_pages) && fits_i32(c.table_width) &&
          (c.head_dim == 64 || c.head_dim == 128) && c.page_size == kCachePage &&
-         c.table_width <= std::numeric_limits<int32_t>::max() / kCachePage &&
+         // (some tokens short of the largest position, so that sums with a page's never pass it)
+         c.table_width <= (std::numeric_limits<int32_t>::max() - 1024) / kCachePage &&
          reinterpret_cast<uintptr_t>(c.key) % 16 == 0 &&
          reinterpret_cast<uintptr_t>(c.value) % 16 == 0;
 }
@@ -74,14 +75,11 @@ __device__ __forceinline__ int physical_page(const CacheQ8& cache, int sequence,
   return page;
 }
 
-// Tokens of a sequence that its table can address; more raise the status bit, fewer than none are
-// none.
+// Tokens of a sequence as given, which its rows' positions follow from; more than its table can
+// address raise the status bit, fewer than none are none.
 __device__ __forceinline__ int sequence_length(const CacheQ8& cache, int sequence, int* status) {
   const int length = max(cache.lengths[sequence], 0);
-  if (length > cache.table_width * kCachePage) {
-    atomicOr(status, NML_SM100_STATUS_INDEX_RANGE);
-    return cache.table_width * kCachePage;
-  }
+  if (length > cache.table_width * kCachePage) atomicOr(status, NML_SM100_STATUS_INDEX_RANGE);
   return length;
 }
 

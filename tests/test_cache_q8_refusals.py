@@ -191,3 +191,10 @@ def test_rotary_table():
             ops.rotary_table(bad, 4)
     with pytest.raises(ValueError):
         ops.rotary_table(frequencies, 0)
+
+
+def test_tables_whose_positions_would_pass_32_bits():
+    for name, request in (("nml_sm100_paged_append_q8", append_request),
+                          ("nml_sm100_paged_read_q8", read_request),
+                          ("nml_sm100_paged_attention_q8", attention_request)):
+        refused(name, request(dict(table_width=2 ** 27 - 64)))

@@ -460,3 +460,35 @@ def test_queries_that_are_not_finite_and_see_nothing(dtype, runs, splits):
     assert status() == _abi.STATUS_INDEX_RANGE
     assert (out[offsets[3]:] == 0).all()
     ref.assert_attention_close(out[:offsets[3]], expected[:offsets[3]], bound[:offsets[3]], dtype)
+
+
+@pytest.mark.parametrize("splits", [1, 2])
+@pytest.mark.parametrize("runs", [False, True])
+def test_lengths_past_the_table_keep_their_positions(runs, splits):
+    """Rows keep the positions that the given length says; of the tokens that they see, those past
+    the table are not there.  A row whose window lies past the table sees its first tokens only."""
+    from nml_b200 import _abi
+    n = 60 if runs else 1
+    for excess in (7, 30, 500, None):
+        lengths, table, cache, query, _, offsets = make(25, torch.bfloat16, 64, 2, 8, [n], [140])
+        full = table.shape[1] * 16
+        given = 2 ** 31 - 1 if excess is None else full + excess
+        for x in cache[0::2]:
+            x.copy_(torch.where(x & 0x7f == 0x7f, 0x30, x))  # every slot of the table is a token's
+        for window, first in ((0, 0), (40, 0), (40, 20)):
+            out = call(query, cache, table, [given], offsets if runs else None, None, splits=splits,
+                       sliding_window=window or None, first_tokens=first)
+            assert status() == _abi.STATUS_INDEX_RANGE
+            for i in range(n):
+                position = given - n + i
+                seen = min(position + 1, full)
+                start = max(0, position + 1 - window) if window else 0
+                if start < seen:
+                    expected, bound = ref.attention(query[i:i + 1], cache, table, [seen], [0, 1],
+                                                    None, seen - start if start else 0, first, 0.125)
+                elif first:
+                    expected, bound = ref.attention(query[i:i + 1], cache, table, [first], [0, 1],
+                                                    None, 0, 0, 0.125)
+                else:
+                    expected = bound = torch.zeros((1, 16, 64), dtype=torch.float64)
+                ref.assert_attention_close(out[i:i + 1], expected, bound, torch.bfloat16)
