@@ -4,14 +4,16 @@
 //   out = sum_j p_j v_j / (sum_j p_j + exp(sink)),  p_j = exp(scale * q.k_j)
 //
 // With k_j = 2^a code_j and v_j = 2^b code'_j (one exponent for each block of 16 tokens) both
-// products run on the bare codes, which are exact in f16:
+// products run on the bare codes, which are exact in f16.  With B the largest value exponent met so
+// far (of a warp) and d = b - B:
 //
-//   t_j = q.code_j * (scale log2(e) 2^a),   w_j = exp2(t_j + b - M),   M = max_j (t_j + b)
-//   numerator = sum_j w_j code'_j,          denominator = sum_j w_j 2^-b
+//   t_j = q.code_j * (scale log2(e) 2^a),   w_j = exp2(t_j + d - M),   M = max_j (t_j + d)
+//   numerator = 2^B sum_j w_j code'_j,      denominator = sum_j w_j 2^-d
 //
 // so a block's scales cost one factor of the scores and one addend of the exponent, and M bounds
-// what actually enters the f16 product.  The exponents lie in [-48, 48]: a weight that underflows
-// (w_j < 2^-126) is below 2^-24 of the denominator's largest term.
+// what enters the f16 product.  Only d from -4 to 2 goes into the f16 weights, whose bits a larger
+// gap would cost: a page below that is weighted with d = 0 and its product scaled by 2^d in f32
+// before it is added, a page above raises B, and the sums so far are scaled once.
 //
 // M is the maximum of the steps before: weights above one are as good as those below as long as F16
 // holds them, so a step's own maximum is formed, and the state rescaled, only when the weights'
@@ -23,8 +25,8 @@
 // one issued as soon as the last read is done, page table entries and scales fetched 32 pages ahead.
 // Scores [16 tokens x 8 heads] = K . q^T with keys widened in registers into mma.sync fragments,
 // weights transposed between lanes by movmatrix, out^T [dims x 8 heads] += V^T . w, where pairs of
-// tokens are interleaved byte-wise before they are widened.  Four CTAs of 112 registers an SM; ten
-// warps an SM keep the conversions and products (about 100 instructions a page) off the memory's
+// tokens are interleaved byte-wise before they are widened.  Four CTAs of 128 registers an SM, sixteen
+// warps, keep the conversions and products (about 100 instructions a page) off the memory's
 // back.  Splits are joined by a second launch that starts while the first still runs.
 //
 // Measured on B200 (device time): 64 sequences of 4097 tokens, 64 query and 8 kv heads of 64 (269.5
@@ -74,7 +76,7 @@ struct RowShape {
 
 // NT: tiles of 8 query heads of one kv head that share the loaded codes.
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 2)
 row_kernel(const AttentionParams p) {
   using S = RowShape<D>;
   constexpr int CP = S::kPages;
@@ -215,6 +217,7 @@ row_kernel(const AttentionParams p) {
 
   float running_max[NT][2], running_sum[NT][2];
   float out[NT][2 * VW][4];  // tile i: dimensions D/8 g + 2i (registers 0, 1) and + 1 (2, 3)
+  float out_exponent = kLowestExponent;  // out is in units of two to this
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     running_max[n][0] = running_max[n][1] = -INFINITY;
@@ -237,15 +240,49 @@ row_kernel(const AttentionParams p) {
     const uint32_t present = there >> at;
     const bool whole = entry >= whole_begin && entry + CP <= whole_end &&
                        (present & ((1u << CP) - 1u)) == (1u << CP) - 1u;
-    float score_factor[NT][CP][2], value_exponent[CP];
+    float score_factor[NT][CP][2];
+    float relative[CP];  // exponent of the page's values, relative to out's
+    bool narrow = true;
 #pragma unroll
     for (int i = 0; i < CP; ++i) {
       const float key_scale = __shfl_sync(0xffffffffu, held.key_scale, at + i);
-      value_exponent[i] = __shfl_sync(0xffffffffu, held.value_exponent, at + i);
+      const float value_exponent = __shfl_sync(0xffffffffu, held.value_exponent, at + i);
+      relative[i] = (present >> i & 1u) != 0 ? value_exponent - out_exponent : 0.0f;
+      narrow = narrow && relative[i] >= kBelowExponent && relative[i] <= kAboveExponent;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         score_factor[n][i][0] = factor[n][0] * key_scale;
         score_factor[n][i][1] = factor[n][1] * key_scale;
+      }
+    }
+    float page_power[CP];  // what a page's products are still to be multiplied by
+    bool wide = false;     // not one for all of them
+    if (__any_sync(0xffffffffu, !narrow)) {
+      float raise = 0.0f;
+#pragma unroll
+      for (int i = 0; i < CP; ++i) {
+        if (relative[i] > kAboveExponent) raise = fmaxf(raise, relative[i]);
+      }
+      out_exponent += raise;
+      const float down = exp2_int(-static_cast<int>(raise));
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < 2 * VW; ++i) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) out[n][i][j] *= down;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < CP; ++i) {
+        if ((present >> i & 1u) != 0) relative[i] -= raise;
+        wide = wide || relative[i] < kBelowExponent;
+      }
+      wide = __any_sync(0xffffffffu, wide);
+#pragma unroll
+      for (int i = 0; i < CP; ++i) {
+        page_power[i] = exp2_int(static_cast<int>(relative[i]));
+        if (wide) relative[i] = 0.0f;
       }
     }
     if (!mbar_wait(&full[warp][slot], k / S::kRing & 1)) {
@@ -322,7 +359,7 @@ row_kernel(const AttentionParams p) {
 #pragma unroll
             for (int i = 0; i < CP; ++i) {
               m = fmaxf(m, fmaf(fmaxf(s[n][i][j], s[n][i][j + 2]), score_factor[n][i][j],
-                                value_exponent[i]));
+                                relative[i]));
             }
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
@@ -350,12 +387,12 @@ row_kernel(const AttentionParams p) {
         }
 #pragma unroll
         for (int i = 0; i < CP; ++i) {
-          const float unscale = exp2_fast(-value_exponent[i]);
+          const float unscale = exp2_fast(-relative[i]);
           float w[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             w[j] = exp2_fast(fmaf(s[n][i][j], score_factor[n][i][j & 1],
-                                  value_exponent[i] - base[j & 1]));
+                                  relative[i] - base[j & 1]));
           }
           largest = fmaxf(largest, fmaxf(w[0] + w[2], w[1] + w[3]));
           step_sum[n][0] = fmaf(w[0] + w[2], unscale, step_sum[n][0]);
@@ -403,25 +440,42 @@ row_kernel(const AttentionParams p) {
           }
         }
       }
+      // two forms of the page's products, so that the common one has no branch in it
+      auto add_products = [&](auto scaled) {
 #pragma unroll
-      for (int w = 0; w < VW; ++w) {
-        const uint32_t lo01 = __byte_perm(values[0][w], values[1][w], 0x5140);
-        const uint32_t lo23 = __byte_perm(values[0][w], values[1][w], 0x7362);
-        const uint32_t hi01 = __byte_perm(values[2][w], values[3][w], 0x5140);
-        const uint32_t hi23 = __byte_perm(values[2][w], values[3][w], 0x7362);
-        const uint32_t a[2][4] = {
-            {e4m3x2_to_f16x2(lo01 & 0xffffu), e4m3x2_to_f16x2(lo01 >> 16),
-             e4m3x2_to_f16x2(hi01 & 0xffffu), e4m3x2_to_f16x2(hi01 >> 16)},
-            {e4m3x2_to_f16x2(lo23 & 0xffffu), e4m3x2_to_f16x2(lo23 >> 16),
-             e4m3x2_to_f16x2(hi23 & 0xffffu), e4m3x2_to_f16x2(hi23 >> 16)}};
+        for (int w = 0; w < VW; ++w) {
+          const uint32_t lo01 = __byte_perm(values[0][w], values[1][w], 0x5140);
+          const uint32_t lo23 = __byte_perm(values[0][w], values[1][w], 0x7362);
+          const uint32_t hi01 = __byte_perm(values[2][w], values[3][w], 0x5140);
+          const uint32_t hi23 = __byte_perm(values[2][w], values[3][w], 0x7362);
+          const uint32_t a[2][4] = {
+              {e4m3x2_to_f16x2(lo01 & 0xffffu), e4m3x2_to_f16x2(lo01 >> 16),
+               e4m3x2_to_f16x2(hi01 & 0xffffu), e4m3x2_to_f16x2(hi01 >> 16)},
+              {e4m3x2_to_f16x2(lo23 & 0xffffu), e4m3x2_to_f16x2(lo23 >> 16),
+               e4m3x2_to_f16x2(hi23 & 0xffffu), e4m3x2_to_f16x2(hi23 >> 16)}};
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
+          for (int n = 0; n < NT; ++n) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            mma_f16(out[n][2 * w + h], a[h][0], a[h][1], a[h][2], a[h][3], weights[n][i][0],
-                    weights[n][i][1]);
+            for (int h = 0; h < 2; ++h) {
+              float(&sum)[4] = out[n][2 * w + h];
+              if constexpr (!decltype(scaled)::value) {
+                mma_f16(sum, a[h][0], a[h][1], a[h][2], a[h][3], weights[n][i][0],
+                        weights[n][i][1]);
+              } else {
+                float product[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                mma_f16(product, a[h][0], a[h][1], a[h][2], a[h][3], weights[n][i][0],
+                        weights[n][i][1]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[j] = fmaf(product[j], page_power[i], sum[j]);
+              }
+            }
           }
         }
+      };
+      if (!wide) {
+        add_products(std::false_type{});
+      } else {
+        add_products(std::true_type{});
       }
     }
     __syncwarp();  // every lane has its codes: the slot is free
@@ -455,6 +509,7 @@ row_kernel(const AttentionParams p) {
       if (g == 0) {
         state[D] = running_max[n][j];
         state[D + 1] = sum;
+        state[D + 2] = out_exponent;
       }
     }
   }
@@ -463,24 +518,29 @@ row_kernel(const AttentionParams p) {
     const int h = item / (D / 4), d0 = 4 * (item % (D / 4));
     const int head = head_base + h;
     if (head >= p.group) continue;
-    float total_max = -INFINITY;
+    float total_max = -INFINITY, exponent = kLowestExponent;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) total_max = fmaxf(total_max, merged[w][h][D]);
+    for (int w = 0; w < kWarps; ++w) {
+      total_max = fmaxf(total_max, merged[w][h][D]);
+      exponent = fmaxf(exponent, merged[w][h][D + 2]);
+    }
     float total_sum = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float m = merged[w][h][D];
       const float weight = m == -INFINITY ? 0.0f : exp2f(m - total_max);
       total_sum += merged[w][h][D + 1] * weight;
+      const float power = weight * exp2_int(static_cast<int>(merged[w][h][D + 2] - exponent));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] = fmaf(merged[w][h][d0 + i], weight, acc[i]);
+      for (int i = 0; i < 4; ++i) acc[i] = fmaf(merged[w][h][d0 + i], power, acc[i]);
     }
     const int64_t query_head = static_cast<int64_t>(row) * p.query_heads + kv_head * p.group + head;
     if (p.splits > 1) {
       float* destination = p.partial + (query_head * p.splits + split) * kStride;
       *reinterpret_cast<float4*>(destination + d0) = make_float4(acc[0], acc[1], acc[2], acc[3]);
       if (d0 == 0) {
-        *reinterpret_cast<float2*>(destination + D) = make_float2(total_max, total_sum);
+        *reinterpret_cast<float4*>(destination + D) =
+            make_float4(total_max, total_sum, exponent, 0.0f);
       }
     } else {
       float denominator = total_sum;
@@ -488,7 +548,8 @@ row_kernel(const AttentionParams p) {
         denominator += exp2f(p.sinks[kv_head * p.group + head] * kLog2e - total_max);
       }
       // only a row that sees nothing has a sum of exactly zero; its output is zero
-      const float inverse = total_sum == 0.0f ? 0.0f : 1.0f / denominator;
+      const float inverse =
+          total_sum == 0.0f ? 0.0f : exp2_int(static_cast<int>(exponent)) / denominator;
       T* out_row = static_cast<T*>(p.output) + query_head * D + d0;
       *reinterpret_cast<uint2*>(out_row) =
           make_uint2(Elem<T>::pack2(acc[0] * inverse, acc[1] * inverse),
@@ -516,24 +577,29 @@ join_kernel(const AttentionParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (nobodys) return;
   const float* base = p.partial + query_head * p.splits * kStride;
-  float total_max = -INFINITY;
-  for (int s = lane; s < p.splits; s += 32) total_max = fmaxf(total_max, base[s * kStride + D]);
+  float total_max = -INFINITY, exponent = kLowestExponent;
+  for (int s = lane; s < p.splits; s += 32) {
+    total_max = fmaxf(total_max, base[s * kStride + D]);
+    exponent = fmaxf(exponent, base[s * kStride + D + 2]);
+  }
 #pragma unroll
   for (int offset = 16; offset > 0; offset >>= 1) {
     total_max = fmaxf(total_max, __shfl_xor_sync(0xffffffffu, total_max, offset));
+    exponent = fmaxf(exponent, __shfl_xor_sync(0xffffffffu, exponent, offset));
   }
   float total_sum = 0.0f, acc[D / 32] = {};
 #pragma unroll 4
   for (int s = warp % kJoinWarps; s < p.splits; s += kJoinWarps) {
     const float* part = base + s * kStride;
-    const float2 state = *reinterpret_cast<const float2*>(part + D);
+    const float4 state = *reinterpret_cast<const float4*>(part + D);
     const float weight = state.x == -INFINITY ? 0.0f : exp2f(state.x - total_max);
     total_sum += state.y * weight;
+    const float power = weight * exp2_int(static_cast<int>(state.z - exponent));
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
       const float2 x = *reinterpret_cast<const float2*>(part + 64 * i + 2 * lane);
-      acc[2 * i] = fmaf(x.x, weight, acc[2 * i]);
-      acc[2 * i + 1] = fmaf(x.y, weight, acc[2 * i + 1]);
+      acc[2 * i] = fmaf(x.x, power, acc[2 * i]);
+      acc[2 * i + 1] = fmaf(x.y, power, acc[2 * i + 1]);
     }
   }
   if constexpr (kJoinWarps > 1) {
@@ -559,7 +625,8 @@ join_kernel(const AttentionParams p) {
   if (p.sinks != nullptr) {
     denominator += exp2f(p.sinks[query_head % p.query_heads] * kLog2e - total_max);
   }
-  const float inverse = total_sum == 0.0f ? 0.0f : 1.0f / denominator;
+  const float inverse =
+      total_sum == 0.0f ? 0.0f : exp2_int(static_cast<int>(exponent)) / denominator;
   T* out = static_cast<T*>(p.output) + query_head * D + 2 * lane;
 #pragma unroll
   for (int i = 0; i < D / 64; ++i) {

@@ -15,13 +15,19 @@ struct AttentionParams {
   const void* query;
   const int32_t* offsets;  // [batch + 1] or null
   const float* sinks;
-  float* partial;          // [rows, query_heads, splits, D + 4]: out, maximum, sum, two unused
+  float* partial;          // [rows, query_heads, splits, D + 4]: out, maximum, sum, exponent, -
   void* output;
   int64_t query_token_stride, query_head_stride;
   int tokens, query_heads, group, head_tiles, splits, window, first;
   float scale_log2;
   int* status;
 };
+
+// Value exponents, relative to the largest one met so far, that weights narrowed to F16 carry:
+// within these, weights of 2^-8 and more of the row's largest keep all their bits and the smallest
+// step is 2^-18 of it.  Pages of smaller values are multiplied by plain weights and their products
+// scaled in f32; larger ones raise the largest and scale what was summed.
+constexpr float kAboveExponent = 2.0f, kBelowExponent = -4.0f;
 
 // Floats of a partial result: a multiple of 16 bytes.
 template <int D>

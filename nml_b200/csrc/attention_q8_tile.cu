@@ -520,7 +520,7 @@ tile_kernel(const AttentionParams p) {
       __syncwarp();
     }
     if (live && p.splits > 1) {
-      *reinterpret_cast<float2*>(partial + D) = make_float2(running_max, running_sum);
+      *reinterpret_cast<float4*>(partial + D) = make_float4(running_max, running_sum, 0.0f, 0.0f);
     }
   } else if (warp >= kMmaWarp) {
     // ------------------------------------------------------------------ matrix products

@@ -140,6 +140,35 @@ def attention(query, cache, table, lengths, offsets, sinks, window, first, scale
     return out, bound
 
 
+def bound_of_each_dimension(query, cache, table, lengths, offsets, sinks, scale):
+    """A bound [tokens, heads, dim] by what each dimension's own values weigh, whatever other tokens
+    hold there: weights narrowed to F16 carry the exponent of their values only from 2^-4 to 2^2 of
+    the largest, so that a probability is off by at most 2^-11 of itself or by half of F16's smallest
+    step, 2^-25, times 2^6, of the row's largest; f32 adds less than 2^-12 of it, as above."""
+    key, key_scales, value, value_scales = cache
+    heads = query.shape[1]
+    group = heads // key.shape[1]
+    bound = torch.zeros(query.shape, dtype=torch.float64)
+    for b, length in enumerate(lengths):
+        begin, end = offsets[b], offsets[b + 1]
+        keys, _, _ = gather(key, key_scales, table[b], length)
+        values, _, _ = gather(value, value_scales, table[b], length)
+        position = torch.arange(begin, end) + (length - end)
+        seen = torch.arange(length)[None] <= position[:, None]
+        for h in range(heads):
+            scores = query[begin:end, h].double() @ keys[:, h // group].T * scale
+            scores = torch.where(seen, scores, -math.inf)
+            p = torch.exp(scores - scores.amax(1, keepdim=True))
+            total = p.sum(1, keepdim=True)
+            if sinks is not None:
+                total = total + torch.exp(sinks[h].double() - scores.amax(1, keepdim=True))
+            off = torch.clamp(p * 2.0 ** -11, min=2.0 ** -19) + p * 2.0 ** -12
+            v = values[:, h // group]
+            bound[begin:end, h] = torch.where(seen, off, 0.0) @ v.abs() / total + \
+                (p @ v / total).abs() * 2.0 ** -12
+    return bound
+
+
 def assert_attention_close(actual, expected, bound, dtype):
     """|a - e| within the bound plus the output's rounding: half a step of its type, or of its
     smallest number."""

@@ -492,3 +492,57 @@ def test_lengths_past_the_table_keep_their_positions(runs, splits):
                 else:
                     expected = bound = torch.zeros((1, 16, 64), dtype=torch.float64)
                 ref.assert_attention_close(out[i:i + 1], expected, bound, torch.bfloat16)
+
+
+def outlier_pages(dim, new, before, gap, at, dtype, seed):
+    """One page of every sequence whose values are 2^gap times the others', in the first half of the
+    dimensions only: the second half is the other pages' alone."""
+    lengths, table, cache, query, sinks, offsets = make(seed, dtype, dim, 2, 8, new, before,
+                                                        with_sinks=True)
+    low = max(127 - 9 - gap // 2, 127 - 48)  # the least exponent that a block has
+    cache[3].fill_(low)
+    for b, length in enumerate(lengths):
+        last = (offsets[b + 1] - offsets[b] + 15) // 16 + 1  # in front of what only some rows see
+        page = int(table[b, {"first": 0, "inside": (length // 16 - last) // 2,
+                             "last": length // 16 - last}[at]])
+        cache[3][page] = low + gap
+        cache[2][page, :, :, dim // 2:] = 0
+    return lengths, table, cache, query * 0.5, sinks, offsets
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("gap", [3, 6, 20, 60, 90])
+@pytest.mark.parametrize("at", ["first", "inside", "last"])
+@pytest.mark.parametrize("splits", [1, 3])
+def test_a_page_of_large_values_takes_nothing_from_the_others(dim, gap, at, splits):
+    new, before = [1, 1, 1], [700, 240, 95]
+    lengths, table, cache, query, sinks, offsets = outlier_pages(dim, new, before, gap, at,
+                                                                 torch.bfloat16, 26)
+    for q in (query, torch.zeros_like(query)):
+        out = call(q, cache, table, lengths, None, sinks, splits=splits)
+        assert status() == 0
+        expected, _ = ref.attention(q, cache, table, lengths, offsets, sinks, 0, 0, dim ** -0.5)
+        bound = ref.bound_of_each_dimension(q, cache, table, lengths, offsets, sinks, dim ** -0.5)
+        assert (bound < 0.05 * expected.abs().amax(-1, keepdim=True)).all()
+        ref.assert_attention_close(out, expected, bound, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("group", [8, 12])
+def test_values_of_every_magnitude(dim, group):
+    """Neighbouring pages up to 2^90 apart, every dimension by its own values."""
+    lengths, table, cache, query, sinks, offsets = make(27, torch.bfloat16, dim, 2, group, [1, 1],
+                                                        [900, 333], with_sinks=True)
+    gen = torch.Generator().manual_seed(27)
+    shape = cache[3].shape
+    cache[3] = torch.randint(127 - 45, 127 + 46, shape, generator=gen).to(torch.uint8)
+    # a dimension holds values of pages of one residue only
+    residue = torch.randint(0, 8, (shape[0], 1, 1, 1), generator=gen)
+    cache[2] = torch.where(torch.arange(dim) % 8 == residue, cache[2], 0)
+    for splits in (1, 2):
+        out = call(query, cache, table, lengths, None, sinks, splits=splits)
+        assert status() == 0
+        expected, _ = ref.attention(query, cache, table, lengths, offsets, sinks, 0, 0, dim ** -0.5)
+        bound = ref.bound_of_each_dimension(query, cache, table, lengths, offsets, sinks,
+                                            dim ** -0.5)
+        ref.assert_attention_close(out, expected, bound, torch.bfloat16)
