@@ -28,6 +28,8 @@ struct AttentionParams {
 // step is 2^-18 of it.  Pages of smaller values are multiplied by plain weights and their products
 // scaled in f32; larger ones raise the largest and scale what was summed.
 constexpr float kAboveExponent = 2.0f, kBelowExponent = -4.0f;
+// (for the tile kernel, which keeps one exponent throughout: of all pages of a walk)
+constexpr int kExponentRange = 6;
 
 // Floats of a partial result: a multiple of 16 bytes.
 template <int D>

@@ -14,7 +14,15 @@
 //              O += W V (A: weights in tensor memory, B: values, MN-major: tokens are rows)
 //   warp 9     brings in the blocks of codes by bulk copies some steps ahead; page table entries
 //              and scales are fetched for 32 pages at a time, 32 pages ahead
+//   warps 10-11  find the range of the pages' value exponents while the others prepare
 // Registers move from the last two warpgroups to the softmax, which holds a row's 64 scores.
+//
+// F16 weights carry the exponents of their values, which costs them bits where these lie far apart.
+// Where the walk's pages lie within 2^6 of each other, as those of one head do, that is bounded (a
+// probability is good to 2^-11 of itself and to 2^-19 of the row's largest); other walks take their
+// values whole, as BF16 (a code times a power of two is exact there), and their weights as the sum
+// of two BF16 terms with a product each.  Ragged prompts take 381 us with both forms in the kernel, 368
+// with the first alone; choosing between them step by step cost 394.
 //
 // The running maximum M only stabilises: weights above one are as good as those below as long as
 // F16 holds them (sums are f32).  So a step is weighted against the maximum of the steps before it,
@@ -46,7 +54,10 @@ constexpr int kStepPages = kStepTokens / kCachePage;
 constexpr int kSoftmaxThreads = 128;
 constexpr int kWidenThreads = 128;
 constexpr int kWidenWarp = 4, kMmaWarp = 8, kLoadWarp = 9;
-constexpr int kThreads = 384;  // the last two warps only give their registers
+constexpr int kThreads = 384;
+constexpr int kRangeWarp = 10, kRangeThreads = 64;
+// named barriers: tensor memory, and the range of exponents for each of the roles that ask for it
+constexpr int kBarrierTmem = 1, kBarrierSoftmax = 2, kBarrierWiden = 3, kBarrierMma = 4;
 constexpr int kLaunchRegisters = 80;  // of a thread: two CTAs fill an SM
 constexpr int kTmemColumns = 256;
 
@@ -95,6 +106,7 @@ struct Control {
   uint32_t tmem;
   int abort_flag;
   int sequence, first_row, rows, first_position;
+  int largest_exponent[kRangeThreads / 32], least_exponent[kRangeThreads / 32];
   PageInfo pages[kInfoSteps][kStepPages];
   alignas(16) uint32_t any_nan[Shape<D>::kStages][4];  // read 16 bytes at a time
   uint8_t row_nan[Shape<D>::kStages][kStepTokens];
@@ -108,6 +120,15 @@ __device__ __forceinline__ void take_registers() {
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
   }
+}
+
+template <int kBarrier, int kCount>
+__device__ __forceinline__ void named_barrier_sync() {
+  asm volatile("barrier.cta.sync.aligned %0, %1;" ::"n"(kBarrier), "n"(kCount) : "memory");
+}
+template <int kBarrier, int kCount>
+__device__ __forceinline__ void named_barrier_arrive() {
+  asm volatile("barrier.cta.arrive.aligned %0, %1;" ::"n"(kBarrier), "n"(kCount) : "memory");
 }
 
 // Two f32 at a time.
@@ -246,7 +267,7 @@ tile_kernel(const AttentionParams p) {
       if (p.sinks != nullptr && live) sink = p.sinks[head] * kLog2e;
     }
     tcgen05_fence_before_sync();
-    asm volatile("barrier.cta.sync.aligned 1, %0;" ::"n"(kSoftmaxThreads + 32) : "memory");
+    named_barrier_sync<kBarrierTmem, kSoftmaxThreads + 32>();
     tcgen05_fence_after_sync();
     tmem = __shfl_sync(0xffffffffu, control.tmem, 0);
   }
@@ -254,6 +275,13 @@ tile_kernel(const AttentionParams p) {
   auto wait = [&](uint64_t* bar, int phase, int site) {
     mbar_wait_or_abort(bar, static_cast<uint32_t>(phase) & 1u, abort_flag, p.status, site);
     __syncwarp();
+  };
+
+  // Whether the walk's values lie too far apart for weights in F16, behind the role's barrier.
+  auto values_far_apart = [&]() {
+    const int range = max(control.largest_exponent[0], control.largest_exponent[1]) -
+                      min(control.least_exponent[0], control.least_exponent[1]);
+    return __any_sync(0xffffffffu, range > kExponentRange) != 0;
   };
 
   // The product of step j.  Whoever has step j's scores knows that the product kBuffers steps
@@ -329,145 +357,168 @@ tile_kernel(const AttentionParams p) {
     // a warp none of whose rows is anybody's hands over whatever its lanes hold: a row of the
     // products depends on that row of weights only
     const bool idle = warp * 32 >= rows * p.group;
-    for (int j = 0; j < steps; ++j) {
-      const int buffer = j % S::kBuffers, stage = j % S::kStages;
-      if (idle) {
+    auto walk = [&](auto whole_values) {
+      constexpr bool kWide = decltype(whole_values)::value;
+      for (int j = 0; j < steps; ++j) {
+        const int buffer = j % S::kBuffers, stage = j % S::kStages;
+        if (idle) {
+          wait(&control.scores_full[buffer], j / S::kBuffers, kSiteScores);
+          mbar_arrive(&control.weights_full[buffer]);
+          continue;
+        }
+        const uint32_t columns = lanes + S::kScores + buffer * kStepTokens;
+        const PageInfo* const pages = control.pages[j % kInfoSteps];
         wait(&control.scores_full[buffer], j / S::kBuffers, kSiteScores);
-        mbar_arrive(&control.weights_full[buffer]);
-        continue;
-      }
-      const uint32_t columns = lanes + S::kScores + buffer * kStepTokens;
-      const PageInfo* const pages = control.pages[j % kInfoSteps];
-      wait(&control.scores_full[buffer], j / S::kBuffers, kSiteScores);
-      tcgen05_fence_after_sync();
-      float page_factor[kStepPages], value_exponent[kStepPages], unscale[kStepPages];
-#pragma unroll
-      for (int q = 0; q < kStepPages; ++q) {
-        const float4 info = *reinterpret_cast<const float4*>(&pages[q]);
-        page_factor[q] = factor * info.x;
-        value_exponent[q] = info.y;
-        unscale[q] = info.z;
-      }
-      const uint4 nan_words = *reinterpret_cast<const uint4*>(control.any_nan[stage]);
-      const bool nans = (nan_words.x | nan_words.y | nan_words.z | nan_words.w) != 0;
-
-      // Weights against the maximum so far; their sum tells whether it still serves.  Only when it
-      // does not (or there is none yet) is the step's maximum formed and the step done again.
-      uint32_t packed[kStepTokens / 2];
-      float step_sum;
-      bool with_maximum = __any_sync(0xffffffffu, running_max == -INFINITY);
-      while (true) {
-        uint32_t scores[2][32];
-        tmem_load_32x32(columns, scores[0]);
-        tmem_load_32x32(columns + 32, scores[1]);
-        tmem_load_wait();
-        float s[kStepTokens];
-#pragma unroll
-        for (int i = 0; i < kStepTokens; ++i) s[i] = __uint_as_float(scores[i / 32][i % 32]);
-        if (j < whole_begin || j >= whole_end || nans) {
-          // bit i: token i is seen; loops, so that the steps without masks branch over all of this
-          uint32_t seen[2] = {0, 0};
-#pragma unroll 1
-          for (int q = 0; q < kStepPages; ++q) {
-            const int t = pages[q].token;
-            auto below = [&](int limit) {  // bits of the page's tokens in front of `limit`
-              return (1u << min(max(limit - t, 0), kCachePage)) - 1u;
-            };
-            const uint32_t bits = below(length) & (~below(start) | below(p.first));
-            if (nans) {
-              const uint8_t* const row_nan = &control.row_nan[stage][q * kCachePage];
-#pragma unroll 1
-              for (int i = 0; i < kCachePage; ++i) {
-                if (row_nan[i] != 0 && (bits >> i & 1u) != 0) poisoned = true;
-              }
-            }
-            const int shift = q * kCachePage & 31;
-            seen[0] |= q < 2 ? bits << shift : 0u;
-            seen[1] |= q < 2 ? 0u : bits << shift;
-          }
-#pragma unroll
-          for (int i = 0; i < kStepTokens; ++i) {
-            if ((seen[i / 32] >> (i % 32) & 1u) == 0) s[i] = -INFINITY;
-          }
-#pragma unroll
-          for (int q = 0; q < kStepPages; ++q) page_factor[q] = masked_factor(page_factor[q]);
-          __syncwarp();
-        }
-        if (with_maximum) {
-          float top = -INFINITY;
-#pragma unroll
-          for (int q = 0; q < kStepPages; ++q) {
-            float m = fmaxf(s[q * kCachePage], s[q * kCachePage + 1]);
-#pragma unroll
-            for (int i = 2; i < kCachePage; i += 2) {
-              m = fmaxf(fmaxf(m, s[q * kCachePage + i]), s[q * kCachePage + i + 1]);
-            }
-            top = fmaxf(top, fmaf(m, page_factor[q], value_exponent[q]));
-          }
-          const bool raise = top > running_max;  // also from -infinity
-          const float next = raise ? top : running_max;
-          const float rescale = raise ? exp2_fast(running_max - next) : 1.0f;
-          if (j > 0) {
-            wait_product(j - 1);
-            tcgen05_fence_after_sync();
-#pragma unroll
-            for (int c = 0; c < D; c += 16) {
-              const uint32_t out_columns = lanes + S::kOut + c;
-              uint32_t x[16], y[8], z[8];
-              tmem_load_32x16(out_columns, x);
-              tmem_load_wait();
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                y[i] = __float_as_uint(__uint_as_float(x[i]) * rescale);
-                z[i] = __float_as_uint(__uint_as_float(x[i + 8]) * rescale);
-              }
-              tmem_store_32x8(out_columns, y);
-              tmem_store_32x8(out_columns + 8, z);
-            }
-          }
-          running_sum *= rescale;
-          running_max = next;
-        }
-        const float base = running_max == -INFINITY ? 0.0f : running_max;
-        step_sum = 0.0f;
-        float largest_sum = 0.0f;
+        tcgen05_fence_after_sync();
+        float page_factor[kStepPages], value_exponent[kStepPages], unscale[kStepPages];
 #pragma unroll
         for (int q = 0; q < kStepPages; ++q) {
-          const float offset = value_exponent[q] - base;
-          const uint64_t factor2 = pack_f32x2(page_factor[q], page_factor[q]);
-          const uint64_t offset2 = pack_f32x2(offset, offset);
-          uint64_t sum2 = 0;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float a, b;
-            unpack_f32x2(fma_f32x2(pack_f32x2(s[q * kCachePage + 2 * i],
-                                              s[q * kCachePage + 2 * i + 1]),
-                                   factor2, offset2),
-                         a, b);
-            a = exp2_fast(a);
-            b = exp2_fast(b);
-            sum2 = add_f32x2(sum2, pack_f32x2(a, b));
-            packed[8 * q + i] = Elem<__half>::pack2(a, b);
-          }
-          float sum_even, sum_odd;
-          unpack_f32x2(sum2, sum_even, sum_odd);
-          const float sum = sum_even + sum_odd;
-          largest_sum = fmaxf(largest_sum, sum);
-          step_sum = fmaf(sum, unscale[q], step_sum);
+          const float4 info = *reinterpret_cast<const float4*>(&pages[q]);
+          page_factor[q] = factor * info.x;
+          // (minus infinity for a page of nobody)
+          value_exponent[q] = !kWide || info.y == -INFINITY ? info.y : 0.0f;
+          unscale[q] = kWide ? 1.0f : info.z;
         }
-        if (with_maximum || !__any_sync(0xffffffffu, largest_sum > kLargestSum)) break;
-        with_maximum = true;
-      }
-      running_sum += step_sum;
-      // over the thread's own scores
+        const uint4 nan_words = *reinterpret_cast<const uint4*>(control.any_nan[stage]);
+        const bool nans = (nan_words.x | nan_words.y | nan_words.z | nan_words.w) != 0;
+
+        // Weights against the maximum so far; their sum tells whether it still serves.  Only when
+        // it does not (or there is none yet) is the step's maximum formed and the step done again.
+        uint32_t packed[kStepTokens / 2], low[kWide ? kStepTokens / 2 : 1];
+        float step_sum;
+        bool with_maximum = __any_sync(0xffffffffu, running_max == -INFINITY);
+        while (true) {
+          uint32_t scores[2][32];
+          tmem_load_32x32(columns, scores[0]);
+          tmem_load_32x32(columns + 32, scores[1]);
+          tmem_load_wait();
+          float s[kStepTokens];
 #pragma unroll
-      for (int q = 0; q < kStepPages; ++q) {
-        const uint32_t(&page)[8] = *reinterpret_cast<const uint32_t(*)[8]>(&packed[8 * q]);
-        tmem_store_32x8(columns + 8 * q, page);
+          for (int i = 0; i < kStepTokens; ++i) s[i] = __uint_as_float(scores[i / 32][i % 32]);
+          if (j < whole_begin || j >= whole_end || nans) {
+            // bit i: token i is seen; loops, so that steps without masks branch over all of this
+            uint32_t seen[2] = {0, 0};
+#pragma unroll 1
+            for (int q = 0; q < kStepPages; ++q) {
+              const int t = pages[q].token;
+              auto below = [&](int limit) {  // bits of the page's tokens in front of `limit`
+                return (1u << min(max(limit - t, 0), kCachePage)) - 1u;
+              };
+              const uint32_t bits = below(length) & (~below(start) | below(p.first));
+              if (nans) {
+                const uint8_t* const row_nan = &control.row_nan[stage][q * kCachePage];
+#pragma unroll 1
+                for (int i = 0; i < kCachePage; ++i) {
+                  if (row_nan[i] != 0 && (bits >> i & 1u) != 0) poisoned = true;
+                }
+              }
+              const int shift = q * kCachePage & 31;
+              seen[0] |= q < 2 ? bits << shift : 0u;
+              seen[1] |= q < 2 ? 0u : bits << shift;
+            }
+#pragma unroll
+            for (int i = 0; i < kStepTokens; ++i) {
+              if ((seen[i / 32] >> (i % 32) & 1u) == 0) s[i] = -INFINITY;
+            }
+#pragma unroll
+            for (int q = 0; q < kStepPages; ++q) page_factor[q] = masked_factor(page_factor[q]);
+            __syncwarp();
+          }
+          if (with_maximum) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int q = 0; q < kStepPages; ++q) {
+              float m = fmaxf(s[q * kCachePage], s[q * kCachePage + 1]);
+#pragma unroll
+              for (int i = 2; i < kCachePage; i += 2) {
+                m = fmaxf(fmaxf(m, s[q * kCachePage + i]), s[q * kCachePage + i + 1]);
+              }
+              top = fmaxf(top, fmaf(m, page_factor[q], value_exponent[q]));
+            }
+            const bool raise = top > running_max;  // also from -infinity
+            const float next = raise ? top : running_max;
+            const float rescale = raise ? exp2_fast(running_max - next) : 1.0f;
+            if (j > 0) {
+              wait_product(j - 1);
+              tcgen05_fence_after_sync();
+#pragma unroll
+              for (int c = 0; c < D; c += 16) {
+                const uint32_t out_columns = lanes + S::kOut + c;
+                uint32_t x[16], y[8], z[8];
+                tmem_load_32x16(out_columns, x);
+                tmem_load_wait();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  y[i] = __float_as_uint(__uint_as_float(x[i]) * rescale);
+                  z[i] = __float_as_uint(__uint_as_float(x[i + 8]) * rescale);
+                }
+                tmem_store_32x8(out_columns, y);
+                tmem_store_32x8(out_columns + 8, z);
+              }
+            }
+            running_sum *= rescale;
+            running_max = next;
+          }
+          const float base = running_max == -INFINITY ? 0.0f : running_max;
+          step_sum = 0.0f;
+          float largest_sum = 0.0f;
+#pragma unroll
+          for (int q = 0; q < kStepPages; ++q) {
+            const float offset = value_exponent[q] - base;
+            const uint64_t factor2 = pack_f32x2(page_factor[q], page_factor[q]);
+            const uint64_t offset2 = pack_f32x2(offset, offset);
+            uint64_t sum2 = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              float a, b;
+              unpack_f32x2(fma_f32x2(pack_f32x2(s[q * kCachePage + 2 * i],
+                                                s[q * kCachePage + 2 * i + 1]),
+                                     factor2, offset2),
+                           a, b);
+              a = exp2_fast(a);
+              b = exp2_fast(b);
+              sum2 = add_f32x2(sum2, pack_f32x2(a, b));
+              if constexpr (kWide) {
+                const uint32_t high = Elem<__nv_bfloat16>::pack2(a, b);
+                packed[8 * q + i] = high;
+                low[8 * q + i] = Elem<__nv_bfloat16>::pack2(
+                    a - __uint_as_float(high << 16), b - __uint_as_float(high & 0xffff0000u));
+              } else {
+                packed[8 * q + i] = Elem<__half>::pack2(a, b);
+              }
+            }
+            float sum_even, sum_odd;
+            unpack_f32x2(sum2, sum_even, sum_odd);
+            const float sum = sum_even + sum_odd;
+            largest_sum = fmaxf(largest_sum, sum);
+            step_sum = fmaf(sum, unscale[q], step_sum);
+          }
+          if (with_maximum || !__any_sync(0xffffffffu, largest_sum > kLargestSum)) break;
+          with_maximum = true;
+        }
+        running_sum += step_sum;
+        // over the thread's own scores
+#pragma unroll
+        for (int q = 0; q < kStepPages; ++q) {
+          const uint32_t(&page)[8] = *reinterpret_cast<const uint32_t(*)[8]>(&packed[8 * q]);
+          tmem_store_32x8(columns + 8 * q, page);
+          if constexpr (kWide) {
+            const uint32_t(&rest)[8] = *reinterpret_cast<const uint32_t(*)[8]>(&low[8 * q]);
+            tmem_store_32x8(columns + kStepTokens / 2 + 8 * q, rest);
+          }
+        }
+        tmem_store_wait();
+        tcgen05_fence_before_sync();
+        mbar_arrive(&control.weights_full[buffer]);
       }
-      tmem_store_wait();
-      tcgen05_fence_before_sync();
-      mbar_arrive(&control.weights_full[buffer]);
+    };
+    if (steps > 0) {
+      named_barrier_sync<kBarrierSoftmax, kRangeThreads + kSoftmaxThreads>();
+      if (values_far_apart()) {
+        walk(std::true_type{});
+      } else {
+        walk(std::false_type{});
+      }
     }
 
     // ---- the rows' results ----
@@ -611,6 +662,8 @@ tile_kernel(const AttentionParams p) {
       constexpr uint32_t score_idesc = umma_idesc_f16(kUmmaF16, kUmmaF16, kTileRows, kStepTokens);
       constexpr uint32_t product_idesc =
           umma_idesc_f16(kUmmaF16, kUmmaF16, kTileRows, D) | (1u << 16);  // B is MN-major
+      constexpr uint32_t wide_idesc =
+          umma_idesc_f16(kUmmaBF16, kUmmaBF16, kTileRows, D) | (1u << 16);
       auto scores = [&](int j) {
         const int stage = j % S::kStages, buffer = j % S::kBuffers;
         wait(&control.tiles_full[stage], j / S::kStages, kSiteTiles);
@@ -633,26 +686,38 @@ tile_kernel(const AttentionParams p) {
         tcgen05_fence_after_sync();
         for (int j = 0; j < min(steps, S::kBuffers); ++j) scores(j);
       }
-      for (int j = 0; j < steps; ++j) {
-        const int stage = j % S::kStages, buffer = j % S::kBuffers;
-        wait(&control.weights_full[buffer], j / S::kBuffers, kSiteWeights);
-        tcgen05_fence_after_sync();
-        const uint32_t values = smem_u32(shared + stage * 2 * S::kTileBytes + S::kTileBytes);
+      auto walk = [&](auto whole_values) {
+        constexpr bool kWide = decltype(whole_values)::value;
+        for (int j = 0; j < steps; ++j) {
+          const int stage = j % S::kStages, buffer = j % S::kBuffers;
+          wait(&control.weights_full[buffer], j / S::kBuffers, kSiteWeights);
+          tcgen05_fence_after_sync();
+          const uint32_t values = smem_u32(shared + stage * 2 * S::kTileBytes + S::kTileBytes);
 #pragma unroll
-        for (int k = 0; k < kStepTokens / 16; ++k) {
-          // 16 tokens are 2 KB of 128-byte rows; the leading offset is the next 64 dimensions' tile
-          const uint32_t address = values + k * 2048;
-          const uint32_t low = ((address & 0x3ffffu) >> 4) | ((kStepTokens * 128 >> 4) << 16);
-          const uint32_t weights = tmem + S::kScores + buffer * kStepTokens + 8 * k;
-          umma_f16_tmem_a_elect(tmem + S::kOut, weights, desc_hi | low, product_idesc,
-                                j > 0 || k > 0 ? 1u : 0u);
+          for (int k = 0; k < (kWide ? 2 : 1) * kStepTokens / 16; ++k) {
+            // 16 tokens are 2 KB of 128-byte rows; the leading offset is the tile of the next 64
+            // dimensions
+            const uint32_t address = values + k % (kStepTokens / 16) * 2048;
+            const uint32_t low = ((address & 0x3ffffu) >> 4) | ((kStepTokens * 128 >> 4) << 16);
+            const uint32_t weights = tmem + S::kScores + buffer * kStepTokens + 8 * k;
+            umma_f16_tmem_a_elect(tmem + S::kOut, weights, desc_hi | low,
+                                  kWide ? wide_idesc : product_idesc, j > 0 || k > 0 ? 1u : 0u);
+          }
+          umma_commit_elect(&control.tiles_free[stage]);
+          umma_commit_elect(&control.product_done[buffer]);
+          if (j + S::kBuffers < steps) {
+            // the scores go over the weights that this product reads
+            wait_product(j);
+            scores(j + S::kBuffers);
+          }
         }
-        umma_commit_elect(&control.tiles_free[stage]);
-        umma_commit_elect(&control.product_done[buffer]);
-        if (j + S::kBuffers < steps) {
-          // the scores go over the weights that this product reads
-          wait_product(j);
-          scores(j + S::kBuffers);
+      };
+      if (steps > 0) {
+        named_barrier_sync<kBarrierMma, kRangeThreads + 32>();
+        if (values_far_apart()) {
+          walk(std::true_type{});
+        } else {
+          walk(std::false_type{});
         }
       }
       umma_commit_elect(&control.drained);
@@ -660,6 +725,45 @@ tile_kernel(const AttentionParams p) {
         *abort_flag = 1;
         atomicOr(p.status, NML_SM100_STATUS_BARRIER_TIMEOUT | (0x100 << kSiteProduct));
       }
+    } else if (steps > 0) {
+      // ---- the range of the walk's value exponents, eight pages of a lane under way at once ----
+      constexpr int kAtOnce = 8;
+      int largest = kLowestExponent, least = kHighestExponent;
+      const int end = min(v.pages, (step_begin + steps) * kStepPages);
+      const int32_t* const table =
+          p.cache.page_table + static_cast<int64_t>(sequence) * p.cache.table_width;
+      for (int i = step_begin * kStepPages + (warp - kRangeWarp) * 32 + lane; i < end;
+           i += kAtOnce * kRangeThreads) {
+        int32_t page[kAtOnce];
+#pragma unroll
+        for (int n = 0; n < kAtOnce; ++n) {
+          const int entry = i + n * kRangeThreads;
+          page[n] = entry < end ? table[entry < v.front ? entry : entry - v.front + v.back] : -1;
+        }
+        int exponent[kAtOnce];
+#pragma unroll
+        for (int n = 0; n < kAtOnce; ++n) {
+          if (page[n] >= p.cache.physical_pages) page[n] = -1;  // (reported by the loads)
+          const int64_t block = static_cast<int64_t>(page[n]) * p.cache.kv_heads + kv_head;
+          exponent[n] = page[n] < 0 ? 0 : scale_exponent(p.cache.scales[1][block]);
+        }
+#pragma unroll
+        for (int n = 0; n < kAtOnce; ++n) {
+          if (page[n] < 0) continue;
+          largest = max(largest, exponent[n]);
+          least = min(least, exponent[n]);
+        }
+      }
+      largest = __reduce_max_sync(0xffffffffu, largest);
+      least = __reduce_min_sync(0xffffffffu, least);
+      if (lane == 0) {
+        control.largest_exponent[warp - kRangeWarp] = largest;
+        control.least_exponent[warp - kRangeWarp] = least;
+      }
+      __syncwarp();
+      named_barrier_arrive<kBarrierWiden, kRangeThreads + kWidenThreads>();
+      named_barrier_arrive<kBarrierMma, kRangeThreads + 32>();
+      named_barrier_arrive<kBarrierSoftmax, kRangeThreads + kSoftmaxThreads>();
     }
   } else {
     // ------------------------------------------------------------------ codes to F16 tiles
@@ -683,40 +787,71 @@ tile_kernel(const AttentionParams p) {
           make_uint4(e4m3x2_to_f16x2(x.z & 0xffffu), e4m3x2_to_f16x2(x.z >> 16),
                      e4m3x2_to_f16x2(x.w & 0xffffu), e4m3x2_to_f16x2(x.w >> 16));
     };
-    for (int j = 0; j < steps; ++j) {
-      const int stage = j % S::kStages, slot = j % S::kStaged;
-      wait(&control.staged_full[slot], j / S::kStaged, kSiteStaged);
-      uint4 keys[kRounds], values[kRounds];
-      int token[kRounds];
-      const uint8_t* const codes = own_codes + slot * 2 * S::kCodeBytes;
+    // a code times a power of two, exact in BF16
+    auto widen_whole = [&](uint8_t* row, const uint4& x, float power) {
+      const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+      uint32_t y[8];
 #pragma unroll
-      for (int r = 0; r < kRounds; ++r) {
-        keys[r] = *reinterpret_cast<const uint4*>(codes + r * kTokens * D);
-        values[r] = *reinterpret_cast<const uint4*>(codes + S::kCodeBytes + r * kTokens * D);
-        token[r] = control.pages[j % kInfoSteps][first_page + r * (kTokens / kCachePage)].token +
-                   first_token % kCachePage;
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t pair = e4m3x2_to_f16x2(words[i / 2] >> (16 * (i & 1)) & 0xffffu);
+        y[i] = Elem<__nv_bfloat16>::pack2(Elem<__half>::from_bits(pair & 0xffffu) * power,
+                                          Elem<__half>::from_bits(pair >> 16) * power);
       }
-      mbar_arrive(&control.staged_free[slot]);
-      if (j >= S::kStages) wait(&control.tiles_free[stage], j / S::kStages - 1, kSiteFree);
-      uint8_t* const tile = own_tile + stage * 2 * S::kTileBytes;
-      bool any_nan = false;
+      *reinterpret_cast<uint4*>(row + chunk_lo) = make_uint4(y[0], y[1], y[2], y[3]);
+      *reinterpret_cast<uint4*>(row + chunk_hi) = make_uint4(y[4], y[5], y[6], y[7]);
+    };
+    auto walk = [&](auto whole_values) {
+      constexpr bool kWide = decltype(whole_values)::value;
+      for (int j = 0; j < steps; ++j) {
+        const int stage = j % S::kStages, slot = j % S::kStaged;
+        wait(&control.staged_full[slot], j / S::kStaged, kSiteStaged);
+        uint4 keys[kRounds], values[kRounds];
+        int token[kRounds];
+        const uint8_t* const codes = own_codes + slot * 2 * S::kCodeBytes;
 #pragma unroll
-      for (int r = 0; r < kRounds; ++r) {
-        // tokens that no row sees, or that are NaN (a whole row of codes then), become zeros; a
-        // page of nobody has negative tokens
-        const bool unseen = token[r] >= v.length || token[r] < 0;
-        const bool nan =
-            ((values[r].x & 0x7fu) == 0x7fu || (keys[r].x & 0x7fu) == 0x7fu) && !unseen;
-        any_nan = any_nan || nan;
-        if (part == 0) control.row_nan[stage][r * kTokens + first_token] = nan ? 1 : 0;
-        if (nan || unseen) keys[r] = values[r] = make_uint4(0, 0, 0, 0);
-        widen(tile + r * kTokens * 128, keys[r]);
-        widen(tile + S::kTileBytes + r * kTokens * 128, values[r]);
+        for (int r = 0; r < kRounds; ++r) {
+          keys[r] = *reinterpret_cast<const uint4*>(codes + r * kTokens * D);
+          values[r] = *reinterpret_cast<const uint4*>(codes + S::kCodeBytes + r * kTokens * D);
+          token[r] = control.pages[j % kInfoSteps][first_page + r * (kTokens / kCachePage)].token +
+                     first_token % kCachePage;
+        }
+        mbar_arrive(&control.staged_free[slot]);
+        if (j >= S::kStages) wait(&control.tiles_free[stage], j / S::kStages - 1, kSiteFree);
+        uint8_t* const tile = own_tile + stage * 2 * S::kTileBytes;
+        bool any_nan = false;
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r) {
+          // tokens that no row sees, or that are NaN (a whole row of codes then), become zeros; a
+          // page of nobody has negative tokens
+          const bool unseen = token[r] >= v.length || token[r] < 0;
+          const bool nan =
+              ((values[r].x & 0x7fu) == 0x7fu || (keys[r].x & 0x7fu) == 0x7fu) && !unseen;
+          any_nan = any_nan || nan;
+          if (part == 0) control.row_nan[stage][r * kTokens + first_token] = nan ? 1 : 0;
+          if (nan || unseen) keys[r] = values[r] = make_uint4(0, 0, 0, 0);
+          widen(tile + r * kTokens * 128, keys[r]);
+          if constexpr (kWide) {
+            const PageInfo& info =
+                control.pages[j % kInfoSteps][first_page + r * (kTokens / kCachePage)];
+            widen_whole(tile + S::kTileBytes + r * kTokens * 128, values[r],
+                        nan || unseen ? 0.0f : exp2_int(static_cast<int>(info.value_exponent)));
+          } else {
+            widen(tile + S::kTileBytes + r * kTokens * 128, values[r]);
+          }
+        }
+        any_nan = __any_sync(0xffffffffu, any_nan);
+        if (lane == 0) control.any_nan[stage][warp - kWidenWarp] = any_nan ? 1u : 0u;
+        fence_proxy_async_smem();
+        mbar_arrive(&control.tiles_full[stage]);
       }
-      any_nan = __any_sync(0xffffffffu, any_nan);
-      if (lane == 0) control.any_nan[stage][warp - kWidenWarp] = any_nan ? 1u : 0u;
-      fence_proxy_async_smem();
-      mbar_arrive(&control.tiles_full[stage]);
+    };
+    if (steps > 0) {
+      named_barrier_sync<kBarrierWiden, kRangeThreads + kWidenThreads>();
+      if (values_far_apart()) {
+        walk(std::true_type{});
+      } else {
+        walk(std::false_type{});
+      }
     }
   }
 

@@ -546,3 +546,40 @@ def test_values_of_every_magnitude(dim, group):
         bound = ref.bound_of_each_dimension(query, cache, table, lengths, offsets, sinks,
                                             dim ** -0.5)
         ref.assert_attention_close(out, expected, bound, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("gap", [3, 6, 20, 60, 90])
+@pytest.mark.parametrize("at", ["first", "inside", "last"])
+@pytest.mark.parametrize("splits", [1, 3])
+def test_a_page_of_large_values_takes_nothing_from_the_others_in_runs(dim, gap, at, splits):
+    new, before = [40, 9, 25], [700, 240, 95]
+    lengths, table, cache, query, sinks, offsets = outlier_pages(dim, new, before, gap, at,
+                                                                 torch.bfloat16, 28)
+    for q in (query, torch.zeros_like(query)):
+        out = call(q, cache, table, lengths, offsets, sinks, splits=splits)
+        assert status() == 0
+        expected, _ = ref.attention(q, cache, table, lengths, offsets, sinks, 0, 0, dim ** -0.5)
+        bound = ref.bound_of_each_dimension(q, cache, table, lengths, offsets, sinks, dim ** -0.5)
+        ref.assert_attention_close(out, expected, bound, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("group", [1, 8, 12])
+def test_values_of_every_magnitude_in_runs(dim, group):
+    new, before = [50, 3, 200], [900, 333, 0]
+    lengths, table, cache, query, sinks, offsets = make(29, torch.bfloat16, dim, 2, group, new,
+                                                        before, with_sinks=True)
+    gen = torch.Generator().manual_seed(29)
+    shape = cache[3].shape
+    cache[3] = torch.randint(127 - 45, 127 + 46, shape, generator=gen).to(torch.uint8)
+    residue = torch.randint(0, 8, (shape[0], 1, 1, 1), generator=gen)
+    cache[2] = torch.where(torch.arange(dim) % 8 == residue, cache[2], 0)
+    # (a slot that no row sees may hold NaN: only the tokens' own dimensions were cleared)
+    for splits in (1, 2):
+        out = call(query, cache, table, lengths, offsets, sinks, splits=splits)
+        assert status() == 0
+        expected, _ = ref.attention(query, cache, table, lengths, offsets, sinks, 0, 0, dim ** -0.5)
+        bound = ref.bound_of_each_dimension(query, cache, table, lengths, offsets, sinks,
+                                            dim ** -0.5)
+        ref.assert_attention_close(out, expected, bound, torch.bfloat16)
