@@ -682,11 +682,11 @@ int32_t nml_sm100_paged_read_q8(const NmlSm100PagedReadQ8 *request, char *error_
  * j > i - sliding_window or j < first_tokens.  `sinks` as in the 16-bit operator.  A row that sees
  * nothing becomes zeros, whatever its queries hold; rows outside every sequence are left as they
  * were.  A row that sees a token becomes NaN when its queries hold an infinity or a NaN, or when a
- * token that it sees is stored as NaN.  Scores, softmax statistics and sums are f32, and scores past
- * f32's range become NaN; queries of BF16 are narrowed to F16 after a power of two for every row that
- * makes this exact down to 2^-29 of the row's largest; probabilities are narrowed to 16 bits, each
- * good to 2^-11 of itself and to 2^-19 of the row's largest, however far apart the magnitudes of the
- * values are. */
+ * token that it sees is stored as NaN.  Scores, softmax statistics and sums are f32 (scores past its
+ * range are not for this operator); queries of BF16 are narrowed to F16 after a power of two for every
+ * row that makes this exact down to 2^-29 of the row's largest; probabilities are narrowed to 16 bits,
+ * each good to 2^-11 of itself and to 2^-19 of the row's largest, however far apart the magnitudes of
+ * the values are. */
 typedef struct NmlSm100PagedAttentionQ8 {
   size_t struct_size;
   NmlSm100CacheQ8 cache;

@@ -18,7 +18,7 @@ Every sequence owns a random set of physical KV pages.
 With ``cache="e4m3"`` the K/V cache is held in 8 bits with a scale for each page and kv head: RoPE
 and the cache write are one launch (``ops.paged_append_q8``) and attention reads half the bytes
 (``ops.paged_attention_q8``); ``DecodeModel.extend`` then also runs several new tokens of every
-sequence at once (prompts, chunks of them, drafted tokens).
+sequence at once (prompts, chunks of them) and keeps them; none can be taken back.
 
 Several GPUs (one process each): sequences are sharded by batch (data-parallel attention, so
 the KV read divides too), experts are sharded with the peer-push schedule of
@@ -300,7 +300,11 @@ class DecodeModel:
     # ------------------------------------------------------------------ the step
     def step(self) -> torch.Tensor:
         """Decodes one token for every sequence of this rank, at the position behind the prior
-        tokens; returns the next token ids."""
+        tokens; returns the next token ids.  The benchmark's step: it is not counted as cached, the
+        next one (or ``extend``) writes over it.  Behind tokens of ``extend`` it is refused: they lie
+        at that position, and ``extend(tokens)`` is what continues from them."""
+        if self.cached != [self.prior] * self.batch:
+            raise ValueError("step decodes behind the prior tokens; extend continues from its own")
         hidden = ops.token_embedding(self.table, self.tokens)
         if self.quantized:
             def attend(layer, q, k, v):
@@ -312,13 +316,15 @@ class DecodeModel:
     def extend(self, tokens: torch.Tensor, counts: list[int] | None = None) -> torch.Tensor:
         """Runs the next ``counts[b]`` tokens of every sequence (one each without ``counts``; a
         sequence may get none) through the model and keeps them in the 8-bit cache.  ``tokens``
-        holds them one sequence after the other; returns the next token id behind each of them."""
+        holds them one sequence after the other; returns the next token id behind each of them.
+        Lengths and offsets come from the host with every call, so a call cannot be captured."""
         if not self.quantized or self.world > 1:
             raise ValueError("extend runs over the e4m3 cache of one rank")
         counts = [1] * self.batch if counts is None else list(counts)
-        if len(counts) != self.batch or min(counts) < 0 or sum(counts) != tokens.numel() or \
-                sum(counts) == 0:
-            raise ValueError("extend expects a count of new tokens for every sequence")
+        if len(counts) != self.batch or min(counts) < 0 or sum(counts) == 0 or \
+                tokens.shape != (sum(counts),):
+            raise ValueError("extend expects a count of new tokens for every sequence, and a vector "
+                             "of the tokens")
         cached = [have + new for have, new in zip(self.cached, counts)]
         if max(cached) > self.capacity:
             raise ValueError(f"the cache has place for {self.capacity} tokens of a sequence")

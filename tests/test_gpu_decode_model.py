@@ -89,3 +89,24 @@ def test_extend_refusals():
         with pytest.raises(ValueError):
             model.extend(tokens[:count], counts)
     assert model.cached == [0, 0]
+
+
+def test_a_step_behind_extended_tokens_is_refused():
+    """The step's position would be one of theirs: nothing of the cache changes."""
+    from nml_b200.decode_step import DecodeModel
+    device = torch.device("cuda")
+    for prior in (0, 9):
+        model = DecodeModel(small_shape(), 2, prior, device, cache="e4m3", room=60)
+        model.step()  # before any token is kept it is what it was
+        tokens = torch.arange(23, dtype=torch.int32, device=device)
+        model.extend(tokens, [20, 3])
+        held = [[x.clone() for x in layer["cache"]] for layer in model.layers]
+        with pytest.raises(ValueError, match="extend"):
+            model.step()
+        torch.cuda.synchronize()
+        for layer, before in zip(model.layers, held):
+            assert all(torch.equal(a, b) for a, b in zip(layer["cache"], before))
+        model.extend(tokens[:2])
+        assert model.cached == [prior + 21, prior + 4]
+        with pytest.raises(ValueError):
+            model.extend(tokens[:4].view(2, 2), [2, 2])
