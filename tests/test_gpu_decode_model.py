@@ -110,3 +110,68 @@ def test_a_step_behind_extended_tokens_is_refused():
         assert model.cached == [prior + 21, prior + 4]
         with pytest.raises(ValueError):
             model.extend(tokens[:4].view(2, 2), [2, 2])
+
+
+def test_attention_of_every_layer_against_the_definition():
+    """What each layer writes and attends to, by the layer's own sinks and window and by lengths that
+    the test counts itself, against the 64-bit definition over the cache that the layer leaves."""
+    from nml_b200 import _abi
+    from nml_b200.decode_step import DecodeModel
+    shape = small_shape()
+    assert shape.sliding_window == 128
+    model = DecodeModel(shape, 3, 0, torch.device("cuda"), cache="e4m3", room=260)
+    seen = []
+    inner = model._append_and_attend
+
+    def record(layer, q, k, v, lengths, offsets):
+        held = [x.cpu() for x in layer["cache"]]
+        out = inner(layer, q, k, v, lengths, offsets)
+        seen.append((layer, q.cpu(), k.cpu(), v.cpu(), held, [x.cpu() for x in layer["cache"]],
+                     out.cpu()))
+        return out
+
+    model._append_and_attend = record
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    table, cached = model.page_table.cpu(), [0, 0, 0]
+    heads, kv_heads, dim = shape.query_heads, shape.key_value_heads, shape.head_dim
+    for counts in ([190, 1, 140], [40, 30, 0], None, None):
+        new = [1, 1, 1] if counts is None else counts
+        tokens = torch.randint(0, shape.vocabulary, (sum(new),), device="cuda", generator=gen,
+                               dtype=torch.int32)
+        seen.clear()
+        model.extend(tokens, counts)
+        torch.cuda.synchronize()
+        assert _abi.device_status(0x1) == 0
+        lengths, offsets = [m + n for m, n in zip(cached, new)], ref.offsets_of(new)
+        position = torch.cat([torch.arange(n) + m for n, m in zip(new, cached)])
+        angles = model.rotary.cpu()[position]
+        assert [id(x[0]) for x in seen] == [id(layer) for layer in model.layers]
+        for index, (layer, q, k, v, before, after, out) in enumerate(seen):
+            rows = [x.view(sum(new), -1, dim).float() for x in (q, k, v)]
+            written = [*ref.append(ref.rotate(rows[1], angles, "half").double(), before[0], before[1],
+                                   table, lengths, offsets),
+                       *ref.append(rows[2].double(), before[2], before[3], table, lengths, offsets)]
+            for got, want in zip(after, written):
+                assert torch.equal(got, want)
+            query = ref.rotate(rows[0], angles, "half").to(torch.bfloat16)
+            expected, bound = ref.attention(query, after, table, lengths, offsets,
+                                            layer["sinks"].cpu(), 128 if index % 2 == 0 else 0, 0,
+                                            dim ** -0.5)
+            ref.assert_attention_close(out.view(sum(new), heads, dim), expected, bound,
+                                       torch.bfloat16)
+        cached = lengths
+    assert model.cached == cached
+    # the benchmark's step behind random prior tokens, where the window has left some behind
+    model = DecodeModel(shape, 2, 150, torch.device("cuda"), cache="e4m3")
+    inner = model._append_and_attend
+    model._append_and_attend = record
+    seen.clear()
+    model.step()
+    for index, (layer, q, _, _, _, after, out) in enumerate(seen):
+        angles = model.rotary.cpu()[150].expand(2, -1)
+        query = ref.rotate(q.view(2, heads, dim).float(), angles, "half").to(torch.bfloat16)
+        expected, bound = ref.attention(query, after, model.page_table.cpu(), [151, 151], [0, 1, 2],
+                                        layer["sinks"].cpu(), 128 if index % 2 == 0 else 0, 0,
+                                        dim ** -0.5)
+        ref.assert_attention_close(out.view(2, heads, dim), expected, bound, torch.bfloat16)
+    assert len(seen) == 2
