@@ -583,3 +583,51 @@ def test_values_of_every_magnitude_in_runs(dim, group):
         bound = ref.bound_of_each_dimension(query, cache, table, lengths, offsets, sinks,
                                             dim ** -0.5)
         ref.assert_attention_close(out, expected, bound, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("splits", [1, 2])
+@pytest.mark.parametrize("dim,kv_heads,group,new,before,window,first,with_sinks",
+                         [case for case in RUNS if sum(case[3]) >= 3 * len(case[3])])
+def test_runs_over_values_far_apart(dtype, dim, kv_heads, group, new, before, window, first,
+                                    with_sinks, splits):
+    """The runs above, for which the tile kernel takes its values whole: neighbouring pages up to 2^16
+    apart.  Weights are two BF16 terms then, off by 2^-17 of themselves: within the bound for F16."""
+    lengths, table, cache, query, sinks, offsets = make(
+        dim + group + 2, dtype, dim, kv_heads, group, new, before, with_sinks=with_sinks)
+    gen = torch.Generator().manual_seed(30)
+    shift = torch.randint(-12, 5, cache[3].shape, generator=gen)
+    cache[3] = (cache[3].int() + shift).to(torch.uint8)
+    out = call(query, cache, table, lengths, offsets, sinks, sliding_window=window or None,
+               first_tokens=first, splits=splits)
+    assert status() == 0
+    expected, bound = ref.attention(query, cache, table, lengths, offsets, sinks, window, first,
+                                    dim ** -0.5)
+    ref.assert_attention_close(out, expected, bound, dtype)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("splits", [1, 2])
+def test_nan_tokens_and_bad_pages_among_values_far_apart(dim, splits):
+    from nml_b200 import _abi
+    lengths, table, cache, query, _, offsets = make(31, torch.bfloat16, dim, 2, 8, [100, 30],
+                                                    [30, 0])
+    cache[3][table[0, 1]] -= 20
+    cache[3][table[1, 0]] += 15
+    for token, at in ((70, 0), (90, 2)):  # a key row of head 0, a value row of head 1
+        page, slot = int(table[0, token // 16]), token % 16
+        cache[at][page, 0 if at == 0 else 1, slot] = 0x7f
+    query[3, 2, 1] = float("nan")
+    expected, bound = ref.attention(torch.nan_to_num(query), cache, table, lengths, offsets, None,
+                                    0, 0, dim ** -0.5)
+    expected[3, 2] = float("nan")
+    out = call(query, cache, table, lengths, offsets, None, splits=splits)
+    assert status() == 0
+    ref.assert_attention_close(out, expected, bound, torch.bfloat16)
+    # rows in front of the first token, and a page of nobody in the middle of the walk
+    table[0, 3] = -1
+    out = call(query, cache, table, [lengths[0], 12], offsets, None, splits=splits)
+    assert status() == _abi.STATUS_INDEX_RANGE
+    assert (out[100:118] == 0).all() and torch.isfinite(out[118:]).all()
+    # rows 0 to 17 see the tokens in front of that page only
+    ref.assert_attention_close(out[:18], expected[:18], bound[:18], torch.bfloat16)
