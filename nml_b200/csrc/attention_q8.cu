@@ -726,7 +726,7 @@ int64_t choose_splits(const NmlSm100PagedAttentionQ8& r) {
 }
 
 bool valid_request(const NmlSm100PagedAttentionQ8& r) {
-  return fits_i32(r.tokens) && r.cache.kv_heads > 0 && r.query_heads > 0 &&
+  return fits_i32(r.tokens) && fits_i32(r.cache.kv_heads) && r.query_heads > 0 &&
          r.query_heads % r.cache.kv_heads == 0 && r.query_heads / r.cache.kv_heads <= 128 &&
          (r.cache.head_dim == 64 || r.cache.head_dim == 128) && fits_i32(r.cache.batch) &&
          fits_i32(r.cache.table_width) && r.splits >= 0 && r.splits <= 64 &&

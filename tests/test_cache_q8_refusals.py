@@ -198,3 +198,9 @@ def test_tables_whose_positions_would_pass_32_bits():
                           ("nml_sm100_paged_read_q8", read_request),
                           ("nml_sm100_paged_attention_q8", attention_request)):
         refused(name, request(dict(table_width=2 ** 27 - 64)))
+
+
+def test_scratch_of_more_heads_than_32_bits_is_not_computed():
+    request = attention_request(dict(kv_heads=2 ** 40), query_heads=2 ** 40)
+    request.struct_size = ctypes.sizeof(request)
+    assert _abi.load().nml_sm100_paged_attention_q8_workspace_bytes(ctypes.byref(request)) == 0
