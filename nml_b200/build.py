@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import argparse
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -24,6 +25,9 @@ SOURCES = ["abi.cu", "embedding.cu", "linear_simt.cu", "linear_umma.cu", "stream
            "cache_q8.cu", "attention_q8.cu",
            "attention_q8_tile.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
+# Kernels whose warps exchange registers count on what a thread has at launch: source -> (part of the
+# kernels' names, registers).  The library refuses to launch them with another count.
+LAUNCH_REGISTERS = {"attention_q8_tile.cu": ("tile_kernel", 80)}
 
 
 def nvcc() -> str:
@@ -31,6 +35,17 @@ def nvcc() -> str:
     if not Path(found).exists():
         raise RuntimeError("nvcc not found; the NVFP4 library cannot be built")
     return found
+
+
+def check_launch_registers(source: str, output: str) -> None:
+    """Fails when the assembler's report on ``source`` gives its kernels other register counts than
+    their shares are written for: here the split can be mended, at run time only be refused."""
+    name, wanted = LAUNCH_REGISTERS[source]
+    found = re.findall(r"entry function '([^']*)'.*?Used (\d+) registers", output, re.DOTALL)
+    counts = {entry: int(count) for entry, count in found if name in entry}
+    if not counts or any(count != wanted for count in counts.values()):
+        raise RuntimeError(f"{source}: {name} must be built with {wanted} registers a thread, the "
+                           f"assembler reports {sorted(counts.values())}")
 
 
 def _stale() -> bool:
@@ -54,13 +69,15 @@ def build(force: bool = False, verbose: bool = False, defines=(), output: Path |
     procs = []
     for source in SOURCES:
         obj = LIB_DIR / (source + (".tuning.o" if defines else ".o"))
+        report = "-v" if verbose or source in LAUNCH_REGISTERS else "-warn-spills"
         cmd = [nvcc(), *ARCH_FLAGS, *[f"-D{d}" for d in defines], "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",
-               "-Xptxas", "-v" if verbose else "-warn-spills", "-c", str(CSRC / source), "-o",
+               "-Xptxas", report, "-c", str(CSRC / source), "-o",
                str(obj)]
         procs.append((source, subprocess.Popen(cmd, stdout=subprocess.PIPE,
                                                stderr=subprocess.STDOUT, text=True)))
         objects.append(str(obj))
     failed = False
+    reports = {}
     for source, proc in procs:
         out, _ = proc.communicate()
         if proc.returncode != 0:
@@ -68,8 +85,11 @@ def build(force: bool = False, verbose: bool = False, defines=(), output: Path |
             sys.stderr.write(f"--- nvcc failed for {source}\n{out}\n")
         elif verbose and out:
             sys.stderr.write(f"--- {source}\n{out}\n")
+        reports[source] = out
     if failed:
         raise RuntimeError("nvcc failed")
+    for source in LAUNCH_REGISTERS:
+        check_launch_registers(source, reports[source])
     link = [nvcc(), *ARCH_FLAGS, "-shared", "-cudart", "static", "-o", str(target), *objects]
     subprocess.run(link, check=True)
     for obj in objects:
