@@ -191,12 +191,13 @@ append_kernel(const AppendParams p) {
     const int lead = position % kCachePage;
     // one lane reads the block's old exponent and, at the end, writes its new one: lanes that run
     // apart could otherwise meet the new one as the old
-    int page = 0, before = kLowestExponent;
+    int page = 0;
+    uint32_t old_scale = 0;  // (below every exponent: no older tokens)
     if (lane == 0) {
       page = physical_page(p.cache, s_sequence[leader], position / kCachePage, p.status);
       if (lead > 0 && page >= 0) {
-        before = scale_exponent((is_key ? p.cache.scales[0] : p.cache.scales[1])
-                                    [static_cast<int64_t>(page) * p.cache.kv_heads + head]);
+        old_scale = (is_key ? p.cache.scales[0] : p.cache.scales[1])
+            [static_cast<int64_t>(page) * p.cache.kv_heads + head];
       }
     }
     const int64_t token_stride = is_key ? p.token_stride[0] : p.token_stride[1];
@@ -250,7 +251,7 @@ append_kernel(const AppendParams p) {
     uint8_t* codes = (is_key ? p.cache.codes[0] : p.cache.codes[1]) + block * (kCachePage * D);
     uint8_t* scale = (is_key ? p.cache.scales[0] : p.cache.scales[1]) + block;
     // tokens in front of the first new row are older ones of this sequence
-    before = __shfl_sync(0xffffffffu, before, 0);
+    const int before = scale_exponent(__shfl_sync(0xffffffffu, old_scale, 0));
     const int exponent = max(block_exponent(largest), before);
     if (lead > 0 && exponent > before) {
       // older codes move to the grown exponent
