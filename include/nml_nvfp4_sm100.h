@@ -597,11 +597,13 @@ size_t nml_sm100_paged_attention_decode_workspace_bytes(int64_t batch, int64_t q
  *
  * Quantisation: the exponent of a block is the smallest e in [-48, 48] with |x| <= 448 * 2^e for
  * every finite row written to it, codes round to nearest even, larger magnitudes saturate.  A
- * token's row of one head that holds an infinity or a NaN is stored as NaN codes throughout.
+ * token's row of one head that holds an infinity or a NaN (of a key: after its rotation) is stored as
+ * NaN codes throughout.
  * Powers of two cost an 8-bit float no precision, and make a block's values exact in 16 bits.
  *
  * Slots that no token was written to may hold anything; a page may be shared by sequences (a
- * common prefix) as long as none of them writes to it.  Page table entries outside
+ * common prefix) as long as none of them writes to it, and stands once in a sequence that does.  Page
+ * table entries outside
  * [0, physical_pages) and lengths beyond table_width pages raise NML_SM100_STATUS_INDEX_RANGE;
  * the tokens concerned are neither written nor visible. */
 typedef struct NmlSm100CacheQ8 {
@@ -661,7 +663,8 @@ int32_t nml_sm100_paged_append_q8(const NmlSm100PagedAppendQ8 *request, char *er
 
 /* Reads the first token_offsets[b + 1] - token_offsets[b] tokens of every sequence back as 16-bit
  * values into rows [token_offsets[b], token_offsets[b + 1]) of the outputs; rows outside every
- * sequence are left as they were, rows behind a bad page table entry become zeros. */
+ * sequence are left as they were, rows behind a bad page table entry become zeros.  F16 outputs are
+ * infinite where a value passes that type's range. */
 typedef struct NmlSm100PagedReadQ8 {
   size_t struct_size;
   NmlSm100CacheQ8 cache;

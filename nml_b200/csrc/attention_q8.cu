@@ -25,13 +25,13 @@
 // one issued as soon as the last read is done, page table entries and scales fetched 32 pages ahead.
 // Scores [16 tokens x 8 heads] = K . q^T with keys widened in registers into mma.sync fragments,
 // weights transposed between lanes by movmatrix, out^T [dims x 8 heads] += V^T . w, where pairs of
-// tokens are interleaved byte-wise before they are widened.  Four CTAs of 128 registers an SM, sixteen
-// warps, keep the conversions and products (about 100 instructions a page) off the memory's
-// back.  Splits are joined by a second launch that starts while the first still runs.
+// tokens are interleaved byte-wise before they are widened.  Four CTAs of 128 registers an SM (13 of
+// their 16 warps on average) keep the conversions and products (about 100 instructions a page) off the
+// memory's back.  Splits are joined by a second launch that starts while the first still runs.
 //
 // Measured on B200 (device time): 64 sequences of 4097 tokens, 64 query and 8 kv heads of 64 (269.5
-// MB): 52.4 us, 5.15 TB/s; 3 sequences of 60000 to 100000 tokens, 32 and 8 heads of 128 (474 MB): 88
-// us, 5.3 TB/s, in 24 splits; one sequence of 413 tokens: 6.4 us.
+// MB): 53.7 us, 5.0 TB/s (58.3 with values far apart); 3 sequences of 60000 to 100000 tokens, 32 and 8
+// heads of 128 (474 MB): 89 us, 5.3 TB/s, in 24 splits; one sequence of 413 tokens: 6.8 us.
 #include <type_traits>
 
 #include "attention_q8.cuh"
@@ -685,7 +685,7 @@ int64_t most_pages(const NmlSm100PagedAttentionQ8& r) {
 
 // Runs of tokens go to the tile kernel, single tokens, and runs of fewer than three on average, to
 // the row kernel.  Measured (8 kv heads of 64, groups of 8): 16 sequences of two rows and 2000 tokens
-// 18 us by rows, 22 by tiles; of four rows 26 and 25; 64 of four rows 86 and 61.
+// 19 us by rows, 22 by tiles; of four rows 26 and 25; 64 of four rows 86 and 61.
 bool use_tiles(const NmlSm100PagedAttentionQ8& r) {
   return r.query_offsets != nullptr && r.tokens >= 3 * r.cache.batch;
 }
@@ -693,11 +693,11 @@ bool use_tiles(const NmlSm100PagedAttentionQ8& r) {
 // Splits of the visible pages: the number with the least estimate of the launch's time, in units of
 // one page of head_dim 64 for a resident CTA of the row kernel (0.19 us): waves of CTAs, each as
 // long as its pages and a fixed part, and what partial results cost to write and join.  At least
-// eight pages each.  Measured on B200 (8 kv heads).  Rows: 64 sequences of 4097 tokens, 52 us
-// unsplit, 59 in two; 128 of 1025, 32 unsplit, 43 in two; 16 of 4097, 18 in four, 32 unsplit; one of
-// 131001, 33 in 64, 901 unsplit; 3 of 60000 to 100000 with head_dim 128, 88 in 24, 129 in 12.  Tiles
+// eight pages each.  Measured on B200 (8 kv heads).  Rows: 64 sequences of 4097 tokens, 53 us
+// unsplit, 59 in two; 128 of 1025, 33 unsplit, 40 in two; 16 of 4097, 19 in four, 34 unsplit; one of
+// 131001, 33 in 64, 953 unsplit; 3 of 60000 to 97000 with head_dim 128, 92 in 24, 133 in 12.  Tiles
 // (an SM's two CTAs take as long as one after the other): one sequence of 64 rows and 4000 tokens,
-// 23 in four, 49 unsplit; 16 of 16 rows and 2000 tokens, 28 unsplit, 32 in two.
+// 23 in four, 47 unsplit; 16 of 16 rows and 2000 tokens, 28 unsplit, 32 in two.
 int64_t choose_splits(const NmlSm100PagedAttentionQ8& r) {
   if (r.splits > 0) return r.splits;
   const int64_t group = r.query_heads / r.cache.kv_heads;

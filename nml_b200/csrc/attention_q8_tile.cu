@@ -21,8 +21,8 @@
 // Where the walk's pages lie within 2^6 of each other, as those of one head do, that is bounded (a
 // probability is good to 2^-11 of itself and to 2^-19 of the row's largest); other walks take their
 // values whole, as BF16 (a code times a power of two is exact there), and their weights as the sum
-// of two BF16 terms with a product each.  Ragged prompts take 381 us with both forms in the kernel, 368
-// with the first alone; choosing between them step by step cost 394.
+// of two BF16 terms with a product each.  The ragged prompts below take 379 us with both forms in the
+// kernel, 366 with the first alone, 459 when they need the second; choosing step by step cost 393.
 //
 // The running maximum M only stabilises: weights above one are as good as those below as long as
 // F16 holds them (sums are f32).  So a step is weighted against the maximum of the steps before it,
@@ -33,8 +33,8 @@
 //
 // What bounds it: one exponential for each score.  A step of 128 x 64 takes 512 clocks of the SM's
 // 16 exponentials per clock and 256 (head_dim 64) of the tensor cores.  Measured on B200: four ragged
-// prompts (1200 to 2000 tokens behind up to 2000, 64 query and 8 kv heads of 64, 197 GFLOP) 360 us,
-// 548 TFLOP/s, half the exponentials' rate.  A CTA's step takes 1490 clocks beside another CTA and
+// prompts (1200 to 2000 tokens behind up to 2000, 64 query and 8 kv heads of 64, 197 GFLOP) 379 us,
+// 520 TFLOP/s, 0.45 of the exponentials' rate.  With the first form alone a CTA's step takes 1490 clocks beside another CTA and
 // 1265 alone: score barrier 100, page data 110, scores 90, exponentials 900 (605 with nothing else on
 // the SM), weights back 120; finding the tile, queries and first codes cost a CTA about 8000, its
 // results 2500.  Tried and slower: polynomial exponentials on the multiply-add units for a quarter

@@ -4,9 +4,10 @@
 // second pass over the data, no atomics.
 //
 // Both are bound by memory (6.46 TB/s measured).  Appending 16384 tokens with 64 query and 8 kv heads
-// of 64, 323 MB: 72 us, 4.5 TB/s (106 with queries and cache writes in one CTA, 173 with every
-// element's partner and angles loaded again); a decode batch of 64: 4.0 us, one of 1: 4.0 us, which
-// is the launch and four dependent loads (length, page, old scale, codes).  Reading back 64 sequences
+// of 64, 323 MB: 74 us, 4.3 TB/s (106 with queries and cache writes in one CTA, 173 with every
+// element's partner and angles loaded again); 4600 tokens with 32 and 8 heads of 128, 77 MB: 37 us, 2.1
+// TB/s, where registers allow two CTAs an SM; a decode batch of 64: 4.1 us, one of 1: 3.8 us, which is
+// the launch and four dependent loads (length, page, old scale, codes).  Reading back 64 sequences
 // of about 4050 tokens, 792 MB: 141 us, 5.6 TB/s.
 #include "cache_q8.cuh"
 

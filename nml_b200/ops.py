@@ -647,9 +647,9 @@ def paged_append_q8(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Ten
     are the last tokens of their sequences, rows ``token_offsets[b] .. token_offsets[b + 1]`` of
     sequence b (I32 [batch + 1]; ``None``: one row each); views of a fused projection's rows are
     fine.  ``sequence_lengths`` counts them in, 0 for an empty place of a padded batch, whose
-    query row becomes zero.  The caches (changed in place) are codes U8 [pages, kv_heads, 16,
+    query row becomes zero; query rows outside every sequence hold anything.  The caches (changed in place) are codes U8 [pages, kv_heads, 16,
     head_dim] and block scales U8 [pages, kv_heads] as ``nml_sm100_paged_append_q8`` describes
-    them; a written page belongs to one sequence.  ``rotary`` is the table of ``rotary_table``
+    them; a written page belongs to one sequence and stands once in its table.  ``rotary`` is the table of ``rotary_table``
     (its width is the rotated part of the head), ``rotary_layout`` pairs elements of the two
     halves (``"half"``) or neighbours (``"interleaved"``)."""
     device = _require_device(key)
@@ -696,7 +696,8 @@ def paged_read_q8(key_cache: torch.Tensor, key_scales: torch.Tensor, value_cache
     """Reads tokens back from the 8-bit paged cache: rows ``token_offsets[b] ..
     token_offsets[b + 1]`` of the two results [tokens, kv_heads, head_dim] are the first tokens of
     sequence b.  ``tokens`` is the results' row count; rows outside every sequence are left as
-    they were (``out``: a pair of contiguous tensors to write into)."""
+    they were in ``out`` (a pair of contiguous tensors to write into) and, without it, hold
+    anything."""
     device = _require_device(key_cache)
     cache = _cache_q8(key_cache, key_scales, value_cache, value_scales, page_table, None, device)
     if token_offsets is None:
@@ -739,7 +740,8 @@ def paged_attention_q8(query: torch.Tensor, key_cache: torch.Tensor, key_scales:
     Every query sees the tokens up to its own; with ``sliding_window`` only the last that many of
     them, and the first ``first_tokens`` of the sequence.  ``sinks`` F32 [query_heads] adds a
     column without a value to the softmax.  A row that sees nothing (an empty place of a padded
-    batch) becomes zeros; rows outside every sequence are left as they were in ``out``.  Scratch
+    batch) becomes zeros; rows outside every sequence are left as they were in ``out`` and, without
+    one, hold anything.  Scratch
     is allocated per call from torch's allocator, so captured graphs never share it."""
     device = _require_device(query)
     if query.dim() != 3:
