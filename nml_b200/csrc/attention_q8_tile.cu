@@ -34,13 +34,14 @@
 // What bounds it: one exponential for each score.  A step of 128 x 64 takes 512 clocks of the SM's
 // 16 exponentials per clock and 256 (head_dim 64) of the tensor cores.  Measured on B200: four ragged
 // prompts (1200 to 2000 tokens behind up to 2000, 64 query and 8 kv heads of 64, 197 GFLOP) 379 us,
-// 520 TFLOP/s, 0.45 of the exponentials' rate.  With the first form alone a CTA's step takes 1490 clocks beside another CTA and
-// 1265 alone: score barrier 100, page data 110, scores 90, exponentials 900 (605 with nothing else on
-// the SM), weights back 120; finding the tile, queries and first codes cost a CTA about 8000, its
-// results 2500.  Tried and slower: polynomial exponentials on the multiply-add units for a quarter
-// or half of the scores (two f32 at a time run there at no more than the rate of one), two threads
-// for a row (437 us where one took 368), three CTAs with the queries in shared memory (446), one CTA
-// of two tiles that share the widened codes and take the exponentials in turn (392).
+// 520 TFLOP/s, 0.45 of the exponentials' rate.  With the first form alone a CTA's step takes 1490
+// clocks beside another CTA and 1265 alone: score barrier 100, page data 110, scores 90, exponentials
+// 900 (605 with nothing else on the SM), weights back 120; finding the tile, queries and first codes
+// cost a CTA about 8000, its results 2500.  Tried and slower: polynomial exponentials on the
+// multiply-add units for a quarter or half of the scores (two f32 at a time run there at no more than
+// the rate of one), two threads for a row (437 us where one took 368), three CTAs with the queries in
+// shared memory (446), one CTA of two tiles that share the widened codes and take the exponentials in
+// turn (392), a short loop over pages for the second form (373, but 757 where it is needed).
 #include <type_traits>
 
 #include "attention_q8.cuh"
