@@ -631,3 +631,87 @@ def test_nan_tokens_and_bad_pages_among_values_far_apart(dim, splits):
     assert (out[100:118] == 0).all() and torch.isfinite(out[118:]).all()
     # rows 0 to 17 see the tokens in front of that page only
     ref.assert_attention_close(out[:18], expected[:18], bound[:18], torch.bfloat16)
+
+
+@pytest.mark.parametrize("runs", [False, True])
+@pytest.mark.parametrize("window", [0, 30])
+def test_tables_wider_than_the_sequences(runs, window):
+    """Entries behind a sequence's last page are not read, whatever they hold; the library chooses
+    splits for the table's width."""
+    new, before = ([30, 1, 7], [200, 20, 0]) if runs else ([1, 1, 1], [229, 20, 6])
+    lengths, table, cache, query, sinks, offsets = make(32, torch.bfloat16, 64, 2, 8, new, before,
+                                                        with_sinks=True)
+    wide = torch.full((3, 4096), -7, dtype=torch.int32)
+    wide[:, 1000:] = 2 ** 31 - 1
+    for b, length in enumerate(lengths):
+        pages = -(-length // 16)
+        wide[b, :pages] = table[b, :pages]
+    out = call(query, cache, wide, lengths, offsets if runs else None, sinks,
+               sliding_window=window or None, first_tokens=3)
+    assert status() == 0
+    expected, bound = ref.attention(query, cache, table, lengths, offsets, sinks, window, 3, 0.125)
+    ref.assert_attention_close(out, expected, bound, torch.bfloat16)
+
+
+@pytest.mark.parametrize("chunk", [60, 150])
+def test_single_tokens_and_a_chunk_in_one_call(chunk):
+    """A chunk of a prompt among the single tokens of a batch: by rows or by tiles as a whole."""
+    new = [1] * 20 + [chunk] + [1] * 11
+    before = [(37 * i) % 300 for i in range(32)]
+    lengths, table, cache, query, sinks, offsets = make(33, torch.float16, 64, 1, 8, new, before,
+                                                        with_sinks=True)
+    out = call(query, cache, table, lengths, offsets, sinks, sliding_window=128)
+    assert status() == 0
+    expected, bound = ref.attention(query, cache, table, lengths, offsets, sinks, 128, 0, 0.125)
+    ref.assert_attention_close(out, expected, bound, torch.float16)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_captured_step_follows_its_buffers(dim):
+    """Append and attention captured once, replayed while lengths, pages and rows change in place: a
+    place is taken, freed and taken again, a block grows, splits have nothing to do at first."""
+    from nml_b200 import ops
+    gen = torch.Generator().manual_seed(34)
+    dtype, kv_heads, group, batch, width = torch.bfloat16, 2, 8, 3, 40
+    heads, pages = kv_heads * group, batch * width
+    start = ref.random_cache(gen, pages, kv_heads, dim)
+    dev = [x.cuda() for x in start]
+    table = torch.randperm(pages, generator=gen).view(batch, width).to(torch.int32)
+    rotary = ops.rotary_table(10000.0 ** (-torch.arange(dim // 2, dtype=torch.float64) / dim), 700)
+    fused = torch.zeros((batch, heads + 2 * kv_heads, dim), dtype=dtype, device="cuda")
+    dev_table, dev_lengths = table.cuda(), torch.zeros(batch, dtype=torch.int32, device="cuda")
+    dev_rotary = rotary.cuda()
+
+    def step():
+        query = ops.paged_append_q8(fused[:, heads:heads + kv_heads], fused[:, heads + kv_heads:],
+                                    *dev, dev_table, dev_lengths, query=fused[:, :heads],
+                                    rotary=dev_rotary)
+        return query, ops.paged_attention_q8(query, *dev, dev_table, dev_lengths, splits=4)
+
+    step()  # every place is empty: nothing is written
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        query, out = step()
+    held = [x.clone() for x in start]
+    for lengths in ([1, 0, 320], [2, 16, 321], [0, 17, 322], [3, 18, 0], [640, 1, 335]):
+        rows = torch.randn(fused.shape, generator=gen) * 2.0 ** (max(lengths) % 5)
+        fused.copy_(rows.to(dtype))
+        dev_lengths.copy_(torch.tensor(lengths, dtype=torch.int32))
+        table = table.flip(0).contiguous()
+        dev_table.copy_(table)
+        graph.replay()
+        assert status() == 0
+        parts = rows.to(dtype).float()
+        angles = rotary[torch.tensor(lengths).clamp(min=1) - 1]
+        offsets = [0, 1, 2, 3]
+        key = ref.rotate(parts[:, heads:heads + kv_heads], angles, "half").double()
+        held = [*ref.append(key, held[0], held[1], table, lengths, offsets),
+                *ref.append(parts[:, heads + kv_heads:].double(), held[2], held[3], table, lengths,
+                            offsets)]
+        for got, want in zip(dev, held):
+            assert torch.equal(got.cpu(), want)
+        expected, bound = ref.attention(query.cpu(), held, table, lengths, offsets, None, 0, 0,
+                                        dim ** -0.5)
+        ref.assert_attention_close(out, expected, bound, dtype)
+        for b in range(batch):
+            assert lengths[b] or (out[b] == 0).all()
