@@ -689,7 +689,7 @@ int32_t nml_sm100_paged_read_q8(const NmlSm100PagedReadQ8 *request, char *error_
  * range are not for this operator); queries of BF16 are narrowed to F16 after a power of two for every
  * row that makes this exact down to 2^-29 of the row's largest; probabilities are narrowed to 16 bits,
  * each good to 2^-11 of itself and to 2^-19 of the row's largest, however far apart the magnitudes of
- * the values are. */
+ * the values are.  The output must not overlap the inputs. */
 typedef struct NmlSm100PagedAttentionQ8 {
   size_t struct_size;
   NmlSm100CacheQ8 cache;

@@ -741,7 +741,7 @@ def paged_attention_q8(query: torch.Tensor, key_cache: torch.Tensor, key_scales:
     them, and the first ``first_tokens`` of the sequence.  ``sinks`` F32 [query_heads] adds a
     column without a value to the softmax.  A row that sees nothing (an empty place of a padded
     batch) becomes zeros; rows outside every sequence are left as they were in ``out`` and, without
-    one, hold anything.  Scratch
+    one, hold anything; ``out`` must not overlap the inputs.  Scratch
     is allocated per call from torch's allocator, so captured graphs never share it."""
     device = _require_device(query)
     if query.dim() != 3:

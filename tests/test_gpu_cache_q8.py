@@ -331,3 +331,34 @@ def test_blocks_that_grow_are_moved_whole(dim, new):
         for got, want in zip(dev, expected):
             assert torch.equal(got.cpu(), want)
     assert status() == 0
+
+
+@pytest.mark.parametrize("rows", [40, 1100])
+def test_more_rows_than_tokens(rows):
+    """Rows in front of a sequence's first token write nothing and give zero queries; the sequence
+    starts at the row of its first token, wherever that lies among the rows."""
+    from nml_b200 import ops
+    gen = torch.Generator().manual_seed(rows)
+    kv_heads, dim, counts = 2, 64, [rows, 5, rows]
+    lengths = [rows - 21, 3, 17]
+    table, pages = ref.random_table(gen, lengths)
+    cache = ref.random_cache(gen, pages, kv_heads, dim)
+    offsets, tokens = ref.offsets_of(counts), 2 * rows + 5
+    key, value = (make_rows(gen, tokens, kv_heads, dim, torch.float16) for _ in range(2))
+    query = make_rows(gen, tokens, 4, dim, torch.float16)
+    rotary = ops.rotary_table(torch.ones(16, dtype=torch.float64) / 3, rows + 1)
+    dev = to_device(cache)
+    out = ops.paged_append_q8(key.cuda(), value.cuda(), *dev, table.cuda(),
+                              torch.tensor(lengths, dtype=torch.int32).cuda(),
+                              torch.tensor(offsets, dtype=torch.int32).cuda(), query=query.cuda(),
+                              rotary=rotary.cuda())
+    assert status() == 0
+    position = torch.cat([torch.arange(n) + m - n for n, m in zip(counts, lengths)])
+    angles = rotary[position.clamp(min=0)]
+    turned = ref.rotate(key.float(), angles, "half").double()
+    expected = [*ref.append(turned, cache[0], cache[1], table, lengths, offsets),
+                *ref.append(value.double(), cache[2], cache[3], table, lengths, offsets)]
+    for got, want in zip(dev, expected):
+        assert torch.equal(got.cpu(), want)
+    rotated = ref.rotate(query.float(), angles, "half").to(torch.float16)
+    assert torch.equal(out.cpu(), torch.where((position >= 0)[:, None, None], rotated, 0))
